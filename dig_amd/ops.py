@@ -256,3 +256,85 @@ def bilinear_ac_into(x, out, c_off):
     _, Ctot, h, w = out.shape
     call("bilinear_ac_concat", **{"in": _chk(x)}, out=out, B=B, H=H, W=W, C=C, h=h, w=w, Ctot=Ctot, c_off=c_off,
          dtype=dtype_code(x.dtype))
+
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _act_code(act, who):
+    if act not in ACTS:
+        raise ValueError(f"{who}: act must be one of {sorted(ACTS)}, got {act!r}")
+    return ACTS[act]
+
+
+def _on_device(who, dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{who}: {name} lives on {t.device} but x on {dev}")
+
+
+def _f32_vec(who, name, t, n):
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be a contiguous float32 tensor of {n} values, got {t.dtype} {tuple(t.shape)}")
+
+
+def _row_strides(t, who, name, lead=1):
+    """Element strides (outer, row) of a channels-last tensor [d0, ..., C] whose leading dimensions from `lead` on step through rows
+    of one pitch (lead = 1: [B, rows, C]; lead = 0: [rows, C] and outer is 0).  Slices of the channels or of the images qualify."""
+    if t.dim() < lead + 1:
+        raise ValueError(f"{who}: {name} needs at least {lead + 1} dimensions, got {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{who}: the channels of {name} must be adjacent in memory (strides {t.stride()})")
+    dims = [(t.shape[i], t.stride(i)) for i in range(lead, t.dim() - 1) if t.shape[i] != 1]
+    for (_, outer), (n, inner) in zip(dims, dims[1:]):
+        if outer != n * inner:
+            raise ValueError(f"{who}: the rows of {name} must have one pitch (shape {tuple(t.shape)}, strides {t.stride()})")
+    ld = dims[-1][1] if dims else t.shape[-1]
+    return (t.stride(0) if lead and t.shape[0] > 1 else 0), ld
+
+
+def _gn_check(who, x, gamma, beta, groups, ss, ss_off):
+    if not x.is_cuda:
+        raise RuntimeError(f"{who} runs on the HIP device only (no CPU fallback): x is on {x.device}")
+    if x.dim() < 2:
+        raise ValueError(f"{who}: x must be [B, ..., C], got {tuple(x.shape)}")
+    dtype_code(x.dtype)
+    B, C = x.shape[0], x.shape[-1]
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"{who}: {C} channels do not divide into {groups} groups")
+    _on_device(who, x.device, gamma=gamma, beta=beta, ss=ss)
+    _f32_vec(who, "gamma", gamma, C)
+    _f32_vec(who, "beta", beta, C)
+    if ss is not None:
+        if ss.dtype != torch.float32 or ss.dim() != 2 or ss.shape[0] != B or ss.stride(1) != 1:
+            raise ValueError(f"{who}: ss must be float32 rows [B, ld] of (scale | shift), got {ss.dtype} {tuple(ss.shape)}")
+        if ss_off < 0 or ss.shape[1] < ss_off + 2 * C:
+            raise ValueError(f"{who}: ss rows of {ss.shape[1]} values do not hold scale and shift of {C} channels at {ss_off}")
+    return B, C, x.numel() // max(1, B * C)
+
+
+def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off=0, res=None, eps=1e-5, want_stats=False):
+    """act(GroupNorm(x) * (1 + scale) + shift) [+ res] of any channels-last tensor x [B, ..., C] (bf16 or fp32; rows of one pitch, e.g.
+    a channel slice): Block.norm / scale-shift / act (ddp.py:158-166) where no conv3x3 left its statistics, any group count.
+    gamma, beta [C] fp32; ss [B, ld] fp32 rows holding (scale | shift) at ss_off; act: none | relu | gelu | silu; res like x.
+    -> y contiguous, in x's type; with want_stats (y, mean_rstd [B, groups, 2] fp32), which train.group_norm_act_bwd takes."""
+    who = "group_norm_act"
+    B, C, P = _gn_check(who, x, gamma, beta, groups, ss, ss_off)
+    code = _act_code(act, who)
+    if not eps > 0:
+        raise ValueError(f"{who}: eps must be positive, got {eps}")
+    if res is not None:
+        _on_device(who, x.device, res=res)
+        if res.shape != x.shape or res.dtype != x.dtype:
+            raise ValueError(f"{who}: res must be like x ({x.dtype} {tuple(x.shape)}), got {res.dtype} {tuple(res.shape)}")
+    x_bs, x_ld = _row_strides(x, who, "x")
+    r_bs, r_ld = _row_strides(res, who, "res") if res is not None else (0, 0)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mr = torch.empty(B, groups, 2, dtype=torch.float32, device=x.device)
+    if out.numel() == 0:  # no pixel: the statistics of nothing are mean 0, variance 0
+        mr[..., 0], mr[..., 1] = 0.0, eps ** -0.5
+        return (out, mr) if want_stats else out
+    ws = torch.empty(B * _lib.lib().dig_gn_act_ws(P, C, groups, 0), dtype=torch.float32, device=x.device)
+    call("gn_act", x=x, gamma=gamma, beta=beta, ss=ss, res=res, out=out, mean_rstd=mr, ws=ws, x_bs=x_bs, x_ld=x_ld, res_bs=r_bs, res_ld=r_ld,
+         B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code, dtype=dtype_code(x.dtype), eps=float(eps))
+    return (out, mr) if want_stats else out

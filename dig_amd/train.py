@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import ops
-from ._lib import call, lib
+from ._lib import call, dtype_code, lib
 from .cam import _layernorm, _pack, _pos_embed
 
 F32 = torch.float32
@@ -94,6 +94,33 @@ def layernorm_bwd(x, gamma, dy, add=None, eps=1e-6):
     call("layernorm_bwd", x=x, gamma=gamma, dy=dy, add=add, dx=dx, part=part, rows=rows, D=D, eps=float(eps))
     gb = colsum(part, nb, 2 * D)
     return dx, gb[:D], gb[D:]
+
+
+def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_off=0):
+    """Adjoint of ops.group_norm_act for x [B, ..., C] and the mean_rstd [B, groups, 2] it returned -> (dx like x, dgamma [C], dbeta [C],
+    dss [B, 2C] = (dscale | dshift) or None without ss), parameter gradients fp32.  The gradient of the residual is dy itself."""
+    who = "group_norm_act_bwd"
+    if mean_rstd.dim() != 3 or mean_rstd.shape[2] != 2 or mean_rstd.dtype != F32 or not mean_rstd.is_contiguous() or mean_rstd.shape[0] != x.shape[0]:
+        raise ValueError(f"{who}: mean_rstd must be the contiguous float32 [B, groups, 2] of the forward, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
+    groups = mean_rstd.shape[1]
+    B, C, P = ops._gn_check(who, x, gamma, beta, groups, ss, ss_off)
+    code = ops._act_code(act, who)
+    ops._on_device(who, x.device, mean_rstd=mean_rstd, dy=dy)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"{who}: dy must be like x ({x.dtype} {tuple(x.shape)}), got {dy.dtype} {tuple(dy.shape)}")
+    x_bs, x_ld = ops._row_strides(x, who, "x")
+    d_bs, d_ld = ops._row_strides(dy, who, "dy")
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    gb = torch.empty(2, C, dtype=F32, device=dev)
+    dss = torch.empty(B, 2 * C, dtype=F32, device=dev) if ss is not None else None
+    if dx.numel() == 0:
+        return dx, gb[0].zero_(), gb[1].zero_(), dss.zero_() if dss is not None else None
+    ws = torch.empty(B * lib().dig_gn_act_ws(P, C, groups, 1), dtype=F32, device=dev)
+    call("gn_act_bwd", x=x, dy=dy, mean_rstd=mean_rstd, gamma=gamma, beta=beta, ss=ss, dx=dx, dgamma=gb[0], dbeta=gb[1], dss=dss, ws=ws, x_bs=x_bs,
+         x_ld=x_ld, dy_bs=d_bs, dy_ld=d_ld, B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code,
+         dtype=dtype_code(x.dtype))
+    return dx, gb[0], gb[1], dss
 
 
 def _dp_apply(u, s, res=None):

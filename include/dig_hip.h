@@ -802,6 +802,54 @@ typedef struct {
 } dig_kd_bin_grad_args;
 int dig_kd_bin_grad(const dig_kd_bin_grad_args* a, void* stream);
 
+/* ---- GroupNorm + scale/shift + activation + residual of a channels-last tensor, and its backward (csrc/gnorm.hip) ---------------
+ * Block / ResnetBlock (ddp.py:151-194) and the LFCA's GroupNorm + ReLU (resnet101.py:31-38) on a tensor that no conv3x3 of this
+ * library wrote statistics for, and in training:
+ *   out = act((x - mean) * rstd * gamma * (1 + scale) + beta * (1 + scale) + shift) [+ res]
+ * x [B][P][C] at b * x_bs + p * x_ld + c (element strides), res likewise, out [B][P][C] contiguous; any C, groups with
+ * C % groups == 0, any alignment (16-byte aligned rows with C % 8 == 0 take 16-byte accesses).
+ *   gamma, beta [C];  ss: per image row b * ss_ld + ss_off: scale [C] | shift [C], or NULL;  act: DIG_ACT_*
+ *   mean_rstd [B][groups][2]: written, what the backward needs;  ws: B * dig_gn_act_ws(P, C, groups, 0) floats */
+#define DIG_ACT_NONE 0
+#define DIG_ACT_RELU 1
+#define DIG_ACT_GELU 2 /* erf form */
+#define DIG_ACT_SILU 3
+typedef struct {
+    const void* x;
+    const float* gamma;
+    const float* beta;
+    const float* ss;
+    const void* res;
+    void* out;
+    float* mean_rstd;
+    float* ws;
+    long long x_bs, x_ld, res_bs, res_ld;
+    int B, P, C, groups, ss_ld, ss_off, act, dtype;
+    float eps;
+} dig_gn_act_args;
+int dig_gn_act(const dig_gn_act_args* a, void* stream);
+/* workspace floats per image of dig_gn_act (bwd = 0) / dig_gn_act_bwd (bwd = 1); negative for a bad shape */
+int dig_gn_act_ws(int P, int C, int groups, int bwd);
+
+/* adjoint: x, dy (strided as above), mean_rstd of the forward -> dx [B][P][C] contiguous, dgamma [C], dbeta [C] and, with ss,
+ * dss [B][2C] = (dscale | dshift).  The residual's gradient is dy itself.  ws: B * dig_gn_act_ws(P, C, groups, 1) floats */
+typedef struct {
+    const void* x;
+    const void* dy;
+    const float* mean_rstd;
+    const float* gamma;
+    const float* beta;
+    const float* ss;
+    void* dx;
+    float* dgamma;
+    float* dbeta;
+    float* dss;
+    float* ws;
+    long long x_bs, x_ld, dy_bs, dy_ld;
+    int B, P, C, groups, ss_ld, ss_off, act, dtype;
+} dig_gn_act_bwd_args;
+int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

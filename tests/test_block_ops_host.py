@@ -1,0 +1,97 @@
+"""Refusals of the channels-last block operators, without a GPU: every one is raised before anything is allocated or launched."""
+import ctypes
+
+import pytest
+import torch
+
+from dig_amd import _lib, ops, train
+
+
+class _Fake(torch.Tensor):
+    """A CPU tensor that claims to live on a HIP device, so that the guards run up to (not into) an allocation."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_subclass(cls, t)
+
+    @property
+    def is_cuda(self):
+        return True
+
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+
+def F(*shape, dtype=torch.float32):
+    return _Fake(torch.zeros(*shape, dtype=dtype))
+
+
+@pytest.fixture(autouse=True)
+def _no_launch(monkeypatch):
+    def refuse(fn, **kw):
+        raise AssertionError(f"dig_{fn} would have been launched")
+
+    monkeypatch.setattr(ops, "call", refuse)
+    monkeypatch.setattr(train, "call", refuse)
+
+
+def test_group_norm_act_refusals():
+    ok = dict(gamma=F(16), beta=F(16), groups=4)
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.group_norm_act(torch.zeros(2, 5, 16), **ok)
+    with pytest.raises(RuntimeError, match="gamma lives on cpu"):
+        ops.group_norm_act(F(2, 5, 16), torch.zeros(16), F(16), groups=4)
+    bad = [(dict(groups=3), "do not divide"), (dict(groups=0), "do not divide"), (dict(act="tanh"), "act must be"), (dict(eps=0.0), "eps must be positive"),
+           (dict(gamma=F(15)), "gamma must be"), (dict(beta=F(16, dtype=torch.bfloat16)), "beta must be"), (dict(gamma=_Fake(torch.zeros(32)[::2])), "gamma must be"),
+           (dict(ss=F(2, 31)), "do not hold"), (dict(ss=F(3, 32)), "ss must be"), (dict(ss=F(2, 40), ss_off=9), "do not hold"), (dict(ss=F(2, 40), ss_off=-1), "do not hold"),
+           (dict(res=F(2, 5, 8)), "res must be"), (dict(res=F(2, 5, 16, dtype=torch.bfloat16)), "res must be")]
+    for kw, msg in bad:
+        with pytest.raises(ValueError, match=msg):
+            ops.group_norm_act(F(2, 5, 16), **dict(ok, **kw))
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        ops.group_norm_act(F(2, 5, 16, dtype=torch.float16), **ok)
+    with pytest.raises(ValueError, match="must be \\[B"):
+        ops.group_norm_act(F(16), **ok)
+    with pytest.raises(ValueError, match="adjacent in memory"):
+        ops.group_norm_act(_Fake(torch.zeros(2, 16, 5).transpose(1, 2)), **ok)
+    with pytest.raises(ValueError, match="one pitch"):
+        ops.group_norm_act(_Fake(torch.zeros(2, 5, 6, 16)[:, :, :4]), **ok)
+
+
+def test_group_norm_act_bwd_refusals():
+    x, ga = F(2, 5, 16), F(16)
+    for mr in (F(2, 4), F(2, 4, 2, dtype=torch.float64), F(3, 4, 2), _Fake(torch.zeros(2, 4, 4)[..., ::2])):
+        with pytest.raises(ValueError, match="mean_rstd must be"):
+            train.group_norm_act_bwd(x, mr, ga, ga, x)
+    with pytest.raises(ValueError, match="do not divide"):
+        train.group_norm_act_bwd(x, F(2, 3, 2), ga, ga, x)
+    with pytest.raises(ValueError, match="dy must be"):
+        train.group_norm_act_bwd(x, F(2, 4, 2), ga, ga, F(2, 5, 16, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="dy lives on cpu"):
+        train.group_norm_act_bwd(x, F(2, 4, 2), ga, ga, torch.zeros(2, 5, 16))
+
+
+def test_gn_act_c_entry_refuses():
+    L = _lib.lib()
+    for fn in ("gn_act", "gn_act_bwd"):
+        S = _lib.STRUCTS[f"dig_{fn}_args"]
+        f = getattr(L, f"dig_{fn}")
+        a = S()
+        assert f(ctypes.byref(a), None) == -1 and b"null pointer" in L.dig_last_error()
+        for name, t in S._fields_:
+            if t is ctypes.c_void_p and name not in ("ss", "res", "dss"):
+                setattr(a, name, 16)
+        for k, v in dict(B=2, P=5, C=16, groups=4, act=3, dtype=0).items():
+            setattr(a, k, v)
+        for k, v, msg in (("groups", 3, b"bad shape"), ("P", 0, b"bad shape"), ("B", -1, b"bad shape"), ("act", 4, b"act 4"), ("dtype", 2, b"dtype 2"),
+                          ("B", (1 << 31) - 1, b"too many blocks")):
+            old = getattr(a, k)
+            setattr(a, k, v)
+            assert f(ctypes.byref(a), None) == -1 and msg in L.dig_last_error(), (fn, k)
+            setattr(a, k, old)
+        a.ss, a.dss = 16, 16
+        if fn == "gn_act":
+            a.ss_ld = 31
+        assert f(ctypes.byref(a), None) == -1 and b"do not hold" in L.dig_last_error()
+    assert L.dig_gn_act_ws(0, 16, 4, 0) < 0 and L.dig_gn_act_ws(5, 16, 3, 0) < 0 and L.dig_gn_act_ws(5, 16, 4, 1) > 0
