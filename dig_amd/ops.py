@@ -338,3 +338,46 @@ def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off
     call("gn_act", x=x, gamma=gamma, beta=beta, ss=ss, res=res, out=out, mean_rstd=mr, ws=ws, x_bs=x_bs, x_ld=x_ld, res_bs=r_bs, res_ld=r_ld,
          B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code, dtype=dtype_code(x.dtype), eps=float(eps))
     return (out, mr) if want_stats else out
+
+
+def _linear_check(who, x, w, bias):
+    if not x.is_cuda:
+        raise RuntimeError(f"{who} runs on the HIP device only (no CPU fallback): x is on {x.device}")
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or w.numel() == 0:
+        raise ValueError(f"{who}: x [..., K] and w [N, K] do not fit: {tuple(x.shape)}, {tuple(w.shape)}")
+    dtype_code(x.dtype)
+    if w.dtype != x.dtype:
+        raise ValueError(f"{who}: x is {x.dtype} but w {w.dtype}")
+    _on_device(who, x.device, w=w, bias=bias)
+    N, K = w.shape
+    if K > 1 and w.stride(1) != 1:
+        raise ValueError(f"{who}: the rows of w must lie with K adjacent (strides {w.stride()})")
+    if bias is not None:
+        _f32_vec(who, "bias", bias, N)
+    return x.numel() // K, N, K
+
+
+def _linear_like(who, name, t, x, N):
+    _on_device(who, x.device, **{name: t})
+    if t.shape != (*x.shape[:-1], N) or t.dtype != x.dtype:
+        raise ValueError(f"{who}: {name} must be {x.dtype} {(*x.shape[:-1], N)}, got {t.dtype} {tuple(t.shape)}")
+    return _row_strides(t, who, name, lead=0)[1]
+
+
+def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
+    """act(x w^T + bias) [+ res]: nn.Linear or a 1x1 convolution of a channels-last tensor, with what follows it, in one launch.
+    x [..., K] (bf16 or fp32; rows of one pitch, e.g. a channel slice), w [N, K] of x's type, bias [N] fp32, act: none | relu | gelu | silu,
+    res [..., N].  -> y [..., N]; with want_pre (y, pre = x w^T + bias in x's type), which train.linear_act_bwd takes."""
+    who = "linear_act"
+    M, N, K = _linear_check(who, x, w, bias)
+    code = _act_code(act, who)
+    ldr = _linear_like(who, "res", res, x, N) if res is not None else 0
+    ldx = _row_strides(x, who, "x", lead=0)[1]
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    pre = torch.empty_like(y) if want_pre else None
+    if M:
+        dt = dtype_code(x.dtype)
+        n = _lib.lib().dig_linear_act_ws(M, N, K, dt)
+        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
+        call("linear_act", x=x, w=w, bias=bias, res=res, out=y, pre=pre, ws=ws, ldx=ldx, ldw=w.stride(0), ldr=ldr, M=M, N=N, K=K, act=code, dtype=dt)
+    return (y, pre) if want_pre else y

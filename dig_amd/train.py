@@ -123,6 +123,31 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     return dx, gb[0], gb[1], dss
 
 
+def linear_act_bwd(x, w, dy, pre=None, act="none", need_dx=True, has_bias=True, dw_f32=False):
+    """Adjoint of ops.linear_act for x [..., K], w [N, K], dy [..., N] and, with an activation, the pre it returned
+    -> (dx like x or None, dw [N, K] in w's type or fp32, db [N] fp32 or None).  The gradient of the residual is dy itself."""
+    who = "linear_act_bwd"
+    M, N, K = ops._linear_check(who, x, w, None)
+    code = ops._act_code(act, who)
+    ldy = ops._linear_like(who, "dy", dy, x, N)
+    if code and pre is None:
+        raise ValueError(f"{who}: act={act!r} needs pre, the pre-activation of the forward (want_pre=True)")
+    ldpre = ops._linear_like(who, "pre", pre, x, N) if code else 0
+    ldx = ops._row_strides(x, who, "x", lead=0)[1]
+    dev, dt = x.device, dtype_code(x.dtype)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+    dw = torch.empty(N, K, dtype=F32 if dw_f32 else w.dtype, device=dev)
+    db = torch.empty(N, dtype=F32, device=dev) if has_bias else None
+    if M == 0:
+        return dx, dw.zero_(), db.zero_() if has_bias else None
+    copy = code or (K % 8 == 0 and (N % 8 or ldy % 8 or dy.data_ptr() % 16))  # dz of its own, rows padded to 8 values
+    dz = torch.empty(M, (N + 7) // 8 * 8, dtype=x.dtype, device=dev) if copy else None
+    ws = torch.empty(lib().dig_linear_act_bwd_ws(M, N, K, dt), dtype=F32, device=dev)
+    call("linear_act_bwd", x=x, w=w, dy=dy, pre=pre if code else None, dx=dx, dw=dw, db=db, dz=dz, ws=ws, ldx=ldx, ldw=w.stride(0), ldy=ldy, ldpre=ldpre,
+         M=M, N=N, K=K, act=code, dtype=dt, dw_f32=int(dw_f32))
+    return dx, dw, db
+
+
 def _dp_apply(u, s, res=None):
     """s_b * u (+ res): a DropPath factor per sample (mask_b / keep_prob) on a branch output u [B, ..., C], as the [B][C][2]
     (scale, shift) table of dig_affine_act_add"""

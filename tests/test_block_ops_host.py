@@ -95,3 +95,57 @@ def test_gn_act_c_entry_refuses():
             a.ss_ld = 31
         assert f(ctypes.byref(a), None) == -1 and b"do not hold" in L.dig_last_error()
     assert L.dig_gn_act_ws(0, 16, 4, 0) < 0 and L.dig_gn_act_ws(5, 16, 3, 0) < 0 and L.dig_gn_act_ws(5, 16, 4, 1) > 0
+
+
+def test_linear_act_refusals():
+    x, w = F(6, 16), F(8, 16)
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.linear_act(torch.zeros(6, 16), w)
+    with pytest.raises(RuntimeError, match="w lives on cpu"):
+        ops.linear_act(x, torch.zeros(8, 16))
+    bad = [(dict(w=F(8, 15)), "do not fit"), (dict(w=F(8, 16, 1)), "do not fit"), (dict(w=F(0, 16)), "do not fit"), (dict(w=F(8, 16, dtype=torch.bfloat16)), "x is"),
+           (dict(w=_Fake(torch.zeros(16, 8).t())), "K adjacent"), (dict(bias=F(7)), "bias must be"), (dict(bias=F(8, dtype=torch.bfloat16)), "bias must be"),
+           (dict(act="elu"), "act must be"), (dict(res=F(6, 7)), "res must be"), (dict(res=F(6, 8, dtype=torch.bfloat16)), "res must be"),
+           (dict(res=_Fake(torch.zeros(8, 6).t())), "adjacent in memory"), (dict(x=_Fake(torch.zeros(4, 3, 2, 16)[:, :, 0][:, :2])), "one pitch")]
+    for kw, msg in bad:
+        with pytest.raises(ValueError, match=msg):
+            ops.linear_act(**dict(dict(x=x, w=w), **kw))
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        ops.linear_act(F(6, 16, dtype=torch.float16), F(8, 16, dtype=torch.float16))
+
+
+def test_linear_act_bwd_refusals():
+    x, w, dy = F(6, 16), F(8, 16), F(6, 8)
+    for kw, msg in ((dict(dy=F(6, 9)), "dy must be"), (dict(act="gelu"), "needs pre"), (dict(act="gelu", pre=F(5, 8)), "pre must be"), (dict(act="x"), "act must be"),
+                    (dict(dy=F(6, 8, dtype=torch.bfloat16)), "dy must be"), (dict(w=F(8, 17)), "do not fit")):
+        with pytest.raises(ValueError, match=msg):
+            train.linear_act_bwd(**dict(dict(x=x, w=w, dy=dy), **kw))
+    with pytest.raises(RuntimeError, match="pre lives on cpu"):
+        train.linear_act_bwd(x, w, dy, act="silu", pre=torch.zeros(6, 8))
+
+
+def test_linear_act_c_entry_refuses():
+    L = _lib.lib()
+    for fn, optional in (("linear_act", ("bias", "res", "pre")), ("linear_act_bwd", ("pre", "dx", "db", "dz"))):
+        S = _lib.STRUCTS[f"dig_{fn}_args"]
+        f = getattr(L, f"dig_{fn}")
+        a = S()
+        assert f(ctypes.byref(a), None) == -1 and b"null pointer" in L.dig_last_error()
+        for name, t in S._fields_:
+            if t is ctypes.c_void_p and name not in optional:
+                setattr(a, name, 16)
+        for k, v in dict(M=6, N=8, K=16, act=0, dtype=0).items():
+            setattr(a, k, v)
+        for k, v, msg in (("M", 0, b"bad shape"), ("N", -1, b"bad shape"), ("K", 0, b"bad shape"), ("K", (1 << 30), b"bad shape"), ("act", 4, b"act 4"), ("act", -1, b"act -1"),
+                          ("dtype", 2, b"dtype 2")):
+            old = getattr(a, k)
+            setattr(a, k, v)
+            assert f(ctypes.byref(a), None) == -1 and msg in L.dig_last_error(), (fn, k, L.dig_last_error())
+            setattr(a, k, old)
+        if fn == "linear_act_bwd":
+            a.act = 2
+            assert f(ctypes.byref(a), None) == -1 and b"needs pre and dz" in L.dig_last_error()
+        else:  # a shape whose k is split needs the workspace
+            a.ws, a.M, a.N, a.K = None, 16, 64, 8192
+            assert L.dig_linear_act_ws(16, 64, 8192, 0) > 0 and f(ctypes.byref(a), None) == -1 and b"needs a workspace" in L.dig_last_error()
+    assert L.dig_linear_act_ws(0, 8, 8, 0) < 0 and L.dig_linear_act_bwd_ws(4, 0, 8, 0) < 0
