@@ -6,6 +6,7 @@ the C declarations.  There is NO fallback: if the library is missing or a call f
 import ctypes
 import os
 import re
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "dig_hip.h")
@@ -81,19 +82,34 @@ def _ptr(x):
     return x.data_ptr()  # torch.Tensor
 
 
-_STRUCT_CACHE = {}
 _SNAME = {"gemm_nt": "dig_gemm_args", "qsample_stem": "dig_stem_args", "bilinear_ac_concat": "dig_bilinear_ac_args",
           "nchw_f32_to_nhwc": "dig_layout_args", "nhwc_to_nchw_f32": "dig_layout_args"}
+_FMT = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_float: "f", ctypes.c_longlong: "q"}
 
 
-def _struct_for(fn):
-    """(ctypes struct class, {field: ctype}) of dig_<fn>'s argument block; built once per entry point (the per-launch host
-    cost is what bounds small batches)."""
-    hit = _STRUCT_CACHE.get(fn)
-    if hit is None:
+class _Entry:
+    """dig_<fn> and how its argument block is packed: one struct.pack of all fields in order (the per-launch host cost is what bounds
+    small batches: setting the fields of a ctypes structure one by one took longer than the rest of a call)."""
+
+    __slots__ = ("slot", "blank", "pack", "func", "sname")
+
+    def __init__(self, fn):
         S = STRUCTS[_SNAME.get(fn, f"dig_{fn}_args")]
-        hit = _STRUCT_CACHE[fn] = (S, dict(S._fields_))
-    return hit
+        self.sname, self.slot, self.blank, fmt = S.__name__, {}, [], ""
+        for name, t in S._fields_:
+            n = getattr(t, "_length_", 0)
+            self.slot[name] = (len(self.blank), n)
+            self.blank += [0] * (n or 1)
+            fmt += _FMT[t._type_] * n if n else _FMT[t]
+        packer = struct.Struct(fmt + "0q")  # native alignment, as the C compiler lays the fields out
+        if packer.size != ctypes.sizeof(S):
+            raise RuntimeError(f"{self.sname}: packed size {packer.size} but the C layout has {ctypes.sizeof(S)}")
+        self.pack = packer.pack
+        self.func = lib()["dig_" + fn]  # a function object of its own: the block goes over as bytes
+        self.func.argtypes, self.func.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+
+
+_ENTRIES = {}
 
 
 TRACE = None  # bench.py's per-launch HIP-event hook: callable(fn, kw, phase) with phase 0 before / 1 after the launch
@@ -106,43 +122,44 @@ def call(fn, stream=None, **kw):
     Raises RuntimeError on a non-zero return."""
     import torch
 
-    L = lib()
+    e = _ENTRIES.get(fn)
+    if e is None:
+        e = _ENTRIES[fn] = _Entry(fn)
     dev = None
+    vals = e.blank[:]
+    slot = e.slot
     for k, v in kw.items():
         if isinstance(v, torch.Tensor):
             if not v.is_cuda:
                 raise RuntimeError(f"dig_{fn}: argument {k!r} is a {v.device} tensor; the kernels take HIP-device pointers only "
                                    "(no CPU fallback) - move the module and its inputs to the device first")
+            d = v.device
             if dev is None:
-                dev = v.device
-            elif v.device != dev:
-                raise RuntimeError(f"dig_{fn}: argument {k!r} lives on {v.device} but another argument on {dev}")
-    S, ftypes = _struct_for(fn)
-    args = S()
-    for k, v in kw.items():
-        ftype = ftypes.get(k)
-        if ftype is None:
-            raise TypeError(f"{S.__name__} has no field {k!r}")
-        if ftype is ctypes.c_void_p:
-            setattr(args, k, v if v is None or isinstance(v, int) else v.data_ptr())
-        elif hasattr(ftype, "_length_"):
-            setattr(args, k, ftype(*v))
-        else:
-            setattr(args, k, v)
+                dev = d
+            elif d != dev:
+                raise RuntimeError(f"dig_{fn}: argument {k!r} lives on {d} but another argument on {dev}")
+            v = v.data_ptr()
+        at = slot.get(k)
+        if at is None:
+            raise TypeError(f"{e.sname} has no field {k!r}")
+        i, n = at
+        if n:
+            for j, x in enumerate(v):
+                vals[i + j] = x
+        elif v is not None:
+            vals[i] = v
+    block = e.pack(*vals)
     tr = TRACE
     if tr is not None:
         tr(fn, kw, 0)
-    if dev is None or dev.index in (None, torch.cuda.current_device()):
-        if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
-        rc = getattr(L, "dig_" + fn)(ctypes.byref(args), ctypes.c_void_p(stream))
+    cur = torch.cuda.current_device()
+    if dev is None or dev.index in (None, cur):
+        rc = e.func(block, torch._C._cuda_getCurrentRawStream(cur) if stream is None else stream)
     else:  # tensors on a device that is not current: the launchers key their per-device state on hipGetDevice()
         with torch.cuda.device(dev):
-            if stream is None:
-                stream = torch.cuda.current_stream(dev).cuda_stream
-            rc = getattr(L, "dig_" + fn)(ctypes.byref(args), ctypes.c_void_p(stream))
+            rc = e.func(block, torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream)
     if rc != 0:
-        raise RuntimeError(f"dig_{fn} failed ({rc}): {L.dig_last_error().decode()}")
+        raise RuntimeError(f"dig_{fn} failed ({rc}): {lib().dig_last_error().decode()}")
     if tr is not None:
         tr(fn, kw, 1)
 

@@ -7,40 +7,31 @@
 // Everything between the loads and the stores is fp32, sums across threads fp64; the only rounding to bf16 is the stored result.
 // No atomics: partial sums lie in the workspace and are added in a fixed order, and how an image is split depends on its own
 // size only, so a result does not depend on the batch it is computed in.
-#include "common.hpp"
+#include "act.hpp"
 
 namespace {
 
 constexpr int NT = 256;
 
-enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
-
-template <int ACT> __device__ __forceinline__ float act_f(float u) {
-    if constexpr (ACT == ACT_RELU) return u < 0.f ? 0.f : u;  // keeps a NaN
-    else if constexpr (ACT == ACT_GELU) return gelu_erf_f(u);
-    else if constexpr (ACT == ACT_SILU) return silu_f(u);
-    else return u;
-}
-template <int ACT> __device__ __forceinline__ float act_d(float u) {
-    if constexpr (ACT == ACT_RELU) return u > 0.f ? 1.f : 0.f;
-    else if constexpr (ACT == ACT_GELU) return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * __expf(-0.5f * u * u) * 0.39894228040143268f;
-    else if constexpr (ACT == ACT_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-u));
-        return s * (1.f + u * (1.f - s));
-    } else return 1.f;
-}
-
-// V consecutive channels of one row (V = 8: 16-byte aligned vectors; V = 1: any alignment)
-template <typename T, int V> __device__ __forceinline__ void vload(float (&f)[V], const T* p) {
-    if constexpr (V == 8) {
-        Frag<T> q;
-        frag_load<T>(q, p);
+// V consecutive channels of one row as they lie in memory (V = 8: 16-byte aligned vectors; V = 1: any alignment)
+template <typename T, int V> struct Raw;
+template <typename T> struct Raw<T, 8> {
+    Frag<T> f;
+    __device__ __forceinline__ void load(const T* p) { frag_load<T>(f, p); }
+    __device__ __forceinline__ void load_once(const T* p) {  // its lines are not kept in the caches
+        f32x4 q[sizeof(T) / 2];
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = frag_get<T>(q, j);
-    } else {
-        f[0] = to_f32<T>(*p);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) q[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p) + i);
+        __builtin_memcpy(&f, q, sizeof(f));
     }
-}
+    __device__ __forceinline__ float get(int j) const { return frag_get<T>(f, j); }
+};
+template <typename T> struct Raw<T, 1> {
+    T f;
+    __device__ __forceinline__ void load(const T* p) { f = *p; }
+    __device__ __forceinline__ void load_once(const T* p) { f = *p; }
+    __device__ __forceinline__ float get(int) const { return to_f32<T>(f); }
+};
 template <typename T, int V> __device__ __forceinline__ void vstore(const float (&f)[V], T* p) {
     if constexpr (V == 8) {
         Frag<T> q;
@@ -49,6 +40,65 @@ template <typename T, int V> __device__ __forceinline__ void vstore(const float 
         frag_store<T>(q, p);
     } else {
         *p = from_f32<T>(f[0]);
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void vstore_once(const float (&f)[V], T* p) {
+    if constexpr (V == 8) {
+        Frag<T> g;
+#pragma unroll
+        for (int j = 0; j < 8; j++) frag_set<T>(g, j, f[j]);
+        f32x4 q[sizeof(T) / 2];
+        __builtin_memcpy(q, &g, sizeof(g));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_nontemporal_store(q[i], reinterpret_cast<f32x4*>(p) + i);
+    } else {
+        *p = from_f32<T>(f[0]);
+    }
+}
+// a thread's n rows, `step` elements apart, U of them in flight: body(vector, row number).  ONCE: the last use of what is read
+template <int U, typename T, int V, bool ONCE = false, typename F> __device__ __forceinline__ void each_row(const T* p, size_t step, int n, F&& body) {
+    int i = 0;
+    for (; i + U <= n; i += U, p += U * step) {
+        Raw<T, V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) ONCE ? v[u].load_once(p + u * step) : v[u].load(p + u * step);
+#pragma unroll
+        for (int u = 0; u < U; u++) body(v[u], i + u);
+    }
+    if (i < n) {
+        Raw<T, V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u < n) ONCE ? v[u].load_once(p + u * step) : v[u].load(p + u * step);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u < n) body(v[u], i + u);
+    }
+}
+template <int U, typename T, int V, bool ONCE = false, typename F>
+__device__ __forceinline__ void each_row2(const T* p, size_t pstep, const T* d, size_t dstep, int n, F&& body) {
+    int i = 0;
+    for (; i + U <= n; i += U, p += U * pstep, d += U * dstep) {
+        Raw<T, V> v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            ONCE ? v[u].load_once(p + u * pstep) : v[u].load(p + u * pstep);
+            ONCE ? w[u].load_once(d + u * dstep) : w[u].load(d + u * dstep);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) body(v[u], w[u], i + u);
+    }
+    if (i < n) {
+        Raw<T, V> v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u < n) {
+                ONCE ? v[u].load_once(p + u * pstep) : v[u].load(p + u * pstep);
+                ONCE ? w[u].load_once(d + u * dstep) : w[u].load(d + u * dstep);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u < n) body(v[u], w[u], i + u);
     }
 }
 
@@ -69,12 +119,14 @@ __host__ __device__ inline Geo geo_of(int P, int C, int G, int V, int rows_per_t
     q.CH = q.LP * V;
     q.nch = (C + q.CH - 1) / q.CH;
     int S = (P + q.R * rows_per_thread - 1) / (q.R * rows_per_thread);
-    if (S > 256) S = 256;
+    if (S > 64) S = 64;
     if (S < 1) S = 1;
     q.RS = (P + S - 1) / S;
     q.S = (P + q.RS - 1) / q.RS;
     return q;
 }
+
+__device__ __forceinline__ int rows_of(int P, int ty, int R) { return P > ty ? (P - ty + R - 1) / R : 0; }
 
 struct FwdP {
     const void* x;
@@ -83,7 +135,7 @@ struct FwdP {
     void* out;
     float *mr, *part;
     long long x_bs, x_ld, r_bs, r_ld;
-    int ss_ld, ss_off;
+    int ss_ld, ss_off, wide;  // wide: gamma, beta and ss can be read 16 bytes at a time
     float eps;
     Geo q;
 };
@@ -99,39 +151,26 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
     const int ch = id % q.nch, b = id / q.nch;
     const int tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
     const int c0 = ch * q.CH, c = c0 + tx * V;
-    const int row0 = s * q.RS, row1 = min(q.P, row0 + q.RS);
+    const int row0 = s * q.R, cycle = q.S * q.R;  // R rows at a time, dealt round over the splits
     const bool on = ty < q.R && c < q.C;
-    const T* x = (const T*)p.x + (size_t)b * p.x_bs + c;
-    float piv[V], s1[V], s2[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) piv[j] = s1[j] = s2[j] = 0.f;
     if (on) {
-        int r = row0 + ty;
-        if (r < row1) vload<T, V>(piv, x + (size_t)r * p.x_ld);
-        for (r += q.R; r + 3 * q.R < row1; r += 4 * q.R) {
-            float f[4][V];
+        const int n = rows_of(q.P, row0 + ty, cycle);
+        const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
+        float piv[V], s1[V], s2[V];
 #pragma unroll
-            for (int u = 0; u < 4; u++) vload<T, V>(f[u], x + (size_t)(r + u * q.R) * p.x_ld);
+        for (int j = 0; j < V; j++) piv[j] = s1[j] = s2[j] = 0.f;
+        each_row<8, T, V>(x, (size_t)cycle * p.x_ld, n, [&](const Raw<T, V>& v, int i) {
+            if (i == 0) {
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = f[u][j] - piv[j];
-                    s1[j] += d;
-                    s2[j] = fmaf(d, d, s2[j]);
-                }
-        }
-        for (; r < row1; r += q.R) {
-            float f[V];
-            vload<T, V>(f, x + (size_t)r * p.x_ld);
+                for (int j = 0; j < V; j++) piv[j] = v.get(j);
+            }
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float d = f[j] - piv[j];
+                const float d = v.get(j) - piv[j];
                 s1[j] += d;
                 s2[j] = fmaf(d, d, s2[j]);
             }
-        }
-        const int len = row1 - row0, n = len > ty ? (len - ty + q.R - 1) / q.R : 0;
+        });
         const float inv = n > 0 ? 1.f / (float)n : 0.f;
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -142,12 +181,12 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
     }
     __syncthreads();
     // groups that meet this chunk, one wave each: weighted mean, then M2 about it
-    const int c1 = min(q.C, c0 + q.CH), g0 = c0 / q.cg, g1 = (c1 - 1) / q.cg, lane = tid & 63, len = row1 - row0;
+    const int c1 = min(q.C, c0 + q.CH), g0 = c0 / q.cg, g1 = (c1 - 1) / q.cg, lane = tid & 63;
     for (int g = g0 + (tid >> 6); g <= g1; g += NT / 64) {
         const int lo = max(c0, g * q.cg) - c0, hi = min(c1, (g + 1) * q.cg) - c0, w = hi - lo;
         double sn = 0.0, sm = 0.0;
         for (int e = lane; e < q.R * w; e += 64) {
-            const int y = e / w, n = len > y ? (len - y + q.R - 1) / q.R : 0;
+            const int y = e / w, n = rows_of(q.P, row0 + y, cycle);
             if (n == 0) continue;
             sm += (double)n * (double)sm_mean[y * q.CH + lo + e - y * w];
             sn += (double)n;
@@ -160,7 +199,7 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
         const double mean = sm / sn;
         double m2 = 0.0;
         for (int e = lane; e < q.R * w; e += 64) {
-            const int y = e / w, n = len > y ? (len - y + q.R - 1) / q.R : 0;
+            const int y = e / w, n = rows_of(q.P, row0 + y, cycle);
             if (n == 0) continue;
             const int i = y * q.CH + lo + e - y * w;
             const double d = (double)sm_mean[i] - mean;
@@ -179,7 +218,7 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
 // rows of split s times channels of group g in chunk ch
 __device__ __forceinline__ double entry_count(const Geo& q, int g, int e) {
     const int ch = e / q.S, s = e - ch * q.S;
-    const int rows = min(q.P, (s + 1) * q.RS) - s * q.RS;
+    const int cycle = q.S * q.R, rows = q.P / cycle * q.R + min(max(q.P % cycle - s * q.R, 0), q.R);
     const int w = min(min(q.C, (ch + 1) * q.CH), (g + 1) * q.cg) - max(ch * q.CH, g * q.cg);
     return w > 0 ? (double)rows * (double)w : 0.0;
 }
@@ -237,39 +276,283 @@ __device__ __forceinline__ void affine_of(const float* gamma, const float* beta,
     }
 }
 
-// ---- pass 3: y = act(gamma' (x - mean) rstd + beta') + res
-template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_apply_kernel(FwdP p) {
-    const Geo q = p.q;
-    int id = blockIdx.x;
-    const int s = id % q.S;
-    id /= q.S;
-    const int ch = id % q.nch, b = id / q.nch;
-    const int tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
-    const int c = ch * q.CH + tx * V;
-    if (ty >= q.R || c >= q.C) return;
-    const int row0 = s * q.RS, row1 = min(q.P, row0 + q.RS);
-    float mean[V], mul[V], add[V];
+// the same for V channels from c, and beta (1 + scale)
+template <int V, typename P> __device__ __forceinline__ void affine_vec(const P& p, int b, int c, float (&a)[V], float (&o)[V], float (&bt)[V]) {
+    float sc[V], sh[V];
+    const float* row = p.ss ? p.ss + (size_t)b * p.ss_ld + p.ss_off + c : nullptr;
+    if (V == 8 && p.wide) {
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        const float* mr = p.mr + ((size_t)b * q.G + (c + j) / q.cg) * 2;
-        float sc;
-        mean[j] = mr[0];
-        affine_of(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, q.C, c + j, mul[j], add[j], sc);
-        mul[j] *= mr[1];
-    }
-    const T* x = (const T*)p.x + (size_t)b * p.x_bs + c;
-    const T* res = p.res ? (const T*)p.res + (size_t)b * p.r_bs + c : nullptr;
-    T* out = (T*)p.out + (size_t)b * q.P * q.C + c;
-    for (int r = row0 + ty; r < row1; r += q.R) {
-        float f[V], h[V];
-        vload<T, V>(f, x + (size_t)r * p.x_ld);
-        if (res) vload<T, V>(h, res + (size_t)r * p.r_ld);
+        for (int h = 0; h < V; h += 4) {
+            *reinterpret_cast<f32x4*>(a + h) = *reinterpret_cast<const f32x4*>(p.gamma + c + h);
+            *reinterpret_cast<f32x4*>(bt + h) = *reinterpret_cast<const f32x4*>(p.beta + c + h);
+            if (row) {
+                *reinterpret_cast<f32x4*>(sc + h) = *reinterpret_cast<const f32x4*>(row + h);
+                *reinterpret_cast<f32x4*>(sh + h) = *reinterpret_cast<const f32x4*>(row + p.q.C + h);
+            }
+        }
+    } else {
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            f[j] = act_f<ACT>(fmaf(f[j] - mean[j], mul[j], add[j]));
-            if (res) f[j] += h[j];
+            a[j] = p.gamma[c + j];
+            bt[j] = p.beta[c + j];
+            if (row) {
+                sc[j] = row[j];
+                sh[j] = row[p.q.C + j];
+            }
         }
-        vstore<T, V>(f, out + (size_t)r * q.C);
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if (row) {
+            const float f = 1.f + sc[j];
+            a[j] *= f;
+            o[j] = fmaf(bt[j], f, sh[j]);
+            bt[j] *= f;
+        } else {
+            o[j] = bt[j];
+        }
+    }
+}
+// the pair [group of channel c + j][2] at `pairs` of V channels
+template <int V> __device__ __forceinline__ void group_pairs(const float* pairs, int cg, int c, float (&x)[V], float (&y)[V]) {
+    if (V == 8 && cg % 8 == 0) {  // c is a multiple of 8: one group
+        const int g = c / cg;
+        const float u = pairs[2 * g], v = pairs[2 * g + 1];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            x[j] = u;
+            y[j] = v;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int g = (c + j) / cg;
+            x[j] = pairs[2 * g];
+            y[j] = pairs[2 * g + 1];
+        }
+    }
+}
+
+// Factors of u = mul (x - mean) + add for the channels of a thread.  For bf16 tensors the mean is folded into add (one instruction less): that
+// costs U |mean| mul of absolute error in u (U = 2^-24), far below the step of x itself.  SiLU's factors are scaled by -log2 e (silu_pre).
+template <typename T, int V, int ACT> struct Affine {
+    static constexpr bool FOLD = sizeof(T) == 2;
+    float mean[FOLD ? 1 : V], mul[V], add[V];
+    __device__ __forceinline__ void set(int j, float m, float mu, float ad) {
+        if constexpr (FOLD) ad = fmaf(-m, mu, ad);
+        else mean[j] = m;
+        mul[j] = ACT == ACT_SILU ? mu * SILU_PRE : mu;
+        add[j] = ACT == ACT_SILU ? ad * SILU_PRE : ad;
+    }
+    __device__ __forceinline__ float value(int j, float x) const {
+        if constexpr (!FOLD) x -= mean[j];
+        if constexpr (ACT == ACT_SILU) return silu_pre(mul[j], add[j], x);
+        else return act_val<T, ACT>(fmaf(x, mul[j], add[j]));
+    }
+};
+
+// ---- pass 3: y = act(gamma' (x - mean) rstd + beta') + res.  With few partials per image (JOIN_MAX) every block joins its groups
+// itself and pass 2 is not launched.
+constexpr int JOIN_GROUPS = 16, JOIN_MAX = 1024;
+// Blocks run from the last image to the first, so that they begin with what pass 1 left in the 256 MB memory-side cache; ONCE (x larger
+// than half of that): loads and stores that are not read again do not displace it.  32x65536x64 bf16 with residual: 227 us without
+// either, 222 reversed, 186 with both.
+template <typename T, int V, int ACT, bool ONCE> __global__ __launch_bounds__(NT) void gn_apply_kernel(FwdP p, int S2, int RS2, int join) {
+    __shared__ float sm_mr[2 * JOIN_GROUPS];
+    const Geo q = p.q;
+    int id = gridDim.x - 1 - blockIdx.x;
+    const int s = id % S2;
+    id /= S2;
+    const int ch = id % q.nch, b = id / q.nch;
+    const int tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
+    const int c0 = ch * q.CH, c = c0 + tx * V, g0 = c0 / q.cg;
+    if (join) {
+        const int g1 = (min(q.C, c0 + q.CH) - 1) / q.cg, lane = tid & 63;
+        for (int g = g0 + (tid >> 6); g <= g1; g += NT / 64) {
+            float m, r;
+            gn_join(p, b, g, lane, m, r);
+            if (lane == 0) {
+                sm_mr[2 * (g - g0)] = m;
+                sm_mr[2 * (g - g0) + 1] = r;
+                if (s == 0) {  // a group that spans chunks is written by each of them: the same value
+                    p.mr[((size_t)b * q.G + g) * 2] = m;
+                    p.mr[((size_t)b * q.G + g) * 2 + 1] = r;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (ty >= q.R || c >= q.C) return;
+    const int row0 = s * RS2, row1 = min(q.P, row0 + RS2);
+    Affine<T, V, ACT> af;
+    {
+        float mean[V], rstd[V], mu[V], ad[V], bt[V];
+        if (join) group_pairs<V>(sm_mr - 2 * g0, q.cg, c, mean, rstd);
+        else group_pairs<V>(p.mr + (size_t)b * q.G * 2, q.cg, c, mean, rstd);
+        affine_vec<V>(p, b, c, mu, ad, bt);
+#pragma unroll
+        for (int j = 0; j < V; j++) af.set(j, mean[j], mu[j] * rstd[j], ad[j]);
+    }
+    const int n = rows_of(row1 - row0, ty, q.R);
+    const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
+    T* out = (T*)p.out + ((size_t)b * q.P + row0 + ty) * q.C + c;
+    const size_t ostep = (size_t)q.R * q.C;
+    if (p.res) {
+        const T* res = (const T*)p.res + (size_t)b * p.r_bs + (size_t)(row0 + ty) * p.r_ld + c;
+        each_row2<4, T, V, ONCE>(x, (size_t)q.R * p.x_ld, res, (size_t)q.R * p.r_ld, n, [&](const Raw<T, V>& v, const Raw<T, V>& h, int) {
+            float y[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) y[j] = af.value(j, v.get(j)) + h.get(j);
+            ONCE ? vstore_once<T, V>(y, out) : vstore<T, V>(y, out);
+            out += ostep;
+        });
+    } else {
+        each_row<4, T, V, ONCE>(x, (size_t)q.R * p.x_ld, n, [&](const Raw<T, V>& v, int) {
+            float y[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) y[j] = af.value(j, v.get(j));
+            ONCE ? vstore_once<T, V>(y, out) : vstore<T, V>(y, out);
+            out += ostep;
+        });
+    }
+}
+
+// ---- one launch: a block owns an image's groups g0 .. g0 + gpc - 1 and keeps all of their pixels in registers (IPT vectors of 8
+// channels per thread): x is read once, no partial sums, no second launch.  Per thread sums about its first row, as above, joined across the block.
+// Consecutive blocks go to the 8 XCDs in turn; the blocks of one image share 128-byte lines where a group's rows are shorter than that, so
+// each XCD (and its L2) gets a contiguous run of them.  Backward 32x4096x256, 64-byte rows: 104 us in plain order, 84 so.
+__device__ __forceinline__ int xcd_run(int id, int n) {
+    const int per = n >> 3, extra = n & 7, x = id & 7;
+    return x * per + min(x, extra) + (id >> 3);
+}
+constexpr int BT = 512;
+struct BGeo {
+    int P, C, G, cg, gpc, nch, LP, R;  // groups per block, blocks per image, vectors per row, rows at a time
+};
+
+template <typename T, int ACT, int IPT> __global__ __launch_bounds__(BT) void gn_block_kernel(FwdP p, BGeo q) {
+    __shared__ float sm_mean[BT * 8], sm_m2[BT * 8];
+    __shared__ float sm_mr[2 * BT];
+    const int id = xcd_run(blockIdx.x, gridDim.x), b = id / q.nch, ch = id - b * q.nch, tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
+    const int g0 = ch * q.gpc, ng = min(q.gpc, q.G - g0), c0 = g0 * q.cg, CH = ng * q.cg, c = c0 + tx * 8;
+    const bool on = ty < q.R && tx * 8 < CH;
+    const bool whole = q.cg % 8 == 0;  // the 8 channels of a vector lie in one group: a thread has one mean, else 8
+    const int pitch = whole ? q.LP : q.LP * 8;
+    Raw<T, 8> f[IPT];
+    const int n = on ? rows_of(q.P, ty, q.R) : 0;
+    if (on) {
+        const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)ty * p.x_ld + c;
+        const size_t step = (size_t)q.R * p.x_ld;
+#pragma unroll
+        for (int k = 0; k < IPT; k++, x += step)
+            if (k < n) f[k].load(x);
+    }
+    float add[8], mul[8];
+    if (on) {
+        float bt[8];
+        affine_vec<8>(p, b, c, mul, add, bt);
+        float m[8], v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) m[j] = v[j] = 0.f;
+#pragma unroll
+        for (int k = 1; k < IPT; k++)
+            if (k < n) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float d = f[k].get(j) - f[0].get(j);
+                    m[j] += d;
+                    v[j] = fmaf(d, d, v[j]);
+                }
+            }
+        if (n > 0) {
+            const float inv = 1.f / (float)n;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float d = m[j] * inv;
+                v[j] -= m[j] * d;
+                m[j] = f[0].get(j) + d;
+            }
+        }
+        if (whole) {
+            const float all = (((m[0] + m[1]) + (m[2] + m[3])) + ((m[4] + m[5]) + (m[6] + m[7]))) * 0.125f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float d = m[j] - all;
+                v[j] = fmaf((float)n * d, d, v[j]);
+            }
+            m[0] = all;
+        }
+        if (whole) {
+            sm_mean[ty * pitch + tx] = m[0];
+            sm_m2[ty * pitch + tx] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                sm_mean[ty * pitch + tx * 8 + j] = m[j];
+                sm_m2[ty * pitch + tx * 8 + j] = v[j];
+            }
+        }
+    }
+    __syncthreads();
+    const int lane = tid & 63, w = whole ? q.cg / 8 : q.cg;  // entries of a group in one row
+    const double n_all = (double)q.P * (double)q.cg;
+    for (int g = tid >> 6; g < ng; g += BT / 64) {
+        double s = 0.0;
+        for (int e = lane; e < q.R * w; e += 64) {
+            const int y = e / w, n = rows_of(q.P, y, q.R);
+            if (n > 0) s += (double)(n * (whole ? 8 : 1)) * (double)sm_mean[y * pitch + g * w + e - y * w];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        const double mean = s / n_all;
+        double m2 = 0.0;
+        for (int e = lane; e < q.R * w; e += 64) {
+            const int y = e / w, n = rows_of(q.P, y, q.R);
+            if (n > 0) {
+                const int i = y * pitch + g * w + e - y * w;
+                const double d = (double)sm_mean[i] - mean;
+                m2 += (double)sm_m2[i] + (double)(n * (whole ? 8 : 1)) * d * d;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m2 += __shfl_xor(m2, o, 64);
+        if (lane == 0) {
+            const float mf = (float)mean, rf = (float)(1.0 / sqrt(m2 / n_all + (double)p.eps));
+            sm_mr[2 * g] = mf;
+            sm_mr[2 * g + 1] = rf;
+            float* o = p.mr + ((size_t)b * q.G + g0 + g) * 2;
+            o[0] = mf;
+            o[1] = rf;
+        }
+    }
+    __syncthreads();
+    if (!on) return;
+    Affine<T, 8, ACT> af;
+    {
+        float mean[8], rstd[8];
+        group_pairs<8>(sm_mr, q.cg, tx * 8, mean, rstd);
+#pragma unroll
+        for (int j = 0; j < 8; j++) af.set(j, mean[j], mul[j] * rstd[j], add[j]);
+    }
+    const size_t rstep = (size_t)q.R * p.r_ld, ostep = (size_t)q.R * q.C;
+    const T* res = p.res ? (const T*)p.res + (size_t)b * p.r_bs + (size_t)ty * p.r_ld + c : nullptr;
+    T* out = (T*)p.out + ((size_t)b * q.P + ty) * q.C + c;
+#pragma unroll
+    for (int k = 0; k < IPT; k++) {
+        if (k < n) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = af.value(j, f[k].get(j));
+            if (res) {
+                Raw<T, 8> h;
+                h.load(res);
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] += h.get(j);
+                res += rstep;
+            }
+            vstore<T, 8>(y, out);
+            out += ostep;
+        }
     }
 }
 
@@ -278,26 +561,35 @@ struct BwdP {
     const void *x, *dy;
     const float *mr, *gamma, *beta, *ss;
     void* dx;
-    float *dgamma, *dbeta, *dss, *part, *sums, *gm;  // part [B][S][C][2], sums [B][C][2] = (S1, S2), gm [B][G][2] = (m1, m2)
+    float *dgamma, *dbeta, *dss;
+    float *part;   // [B][S][C][2]: S1, S2 of a split's rows
+    float *gpart;  // [B][G][nch S][2]: sums over the group's channels in the chunk of gamma' S1, gamma' S2
+    float* gm;     // [B][G][2]: m1, m2, where the blocks do not join their groups themselves
     long long x_bs, x_ld, d_bs, d_ld;
-    int ss_ld, ss_off, B;
+    int ss_ld, ss_off, wide, B;
     Geo q;
 };
 
-// What one channel needs for du: u = mul (x - mean) + add.
+// What one channel needs for du = dy act'(u), u = mul (x - mean) + add (SiLU: mul and add scaled by -log2 e)
 struct ChanB {
     float mean, rstd, mul, add, tol;  // tol: below it the sign of u is not certain in fp32
 };
-__device__ __forceinline__ ChanB chan_b(const BwdP& p, int b, int c) {
-    const float* mr = p.mr + ((size_t)b * p.q.G + c / p.q.cg) * 2;
-    ChanB k;
-    float sc;
-    k.mean = mr[0];
-    k.rstd = mr[1];
-    affine_of(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, p.q.C, c, k.mul, k.add, sc);
-    k.mul *= k.rstd;
-    k.tol = 1e-5f * (fabsf(p.beta[c] * sc) + fabsf(k.add - p.beta[c] * sc));
-    return k;
+template <int ACT, int V> __device__ __forceinline__ void chan_b(const BwdP& p, int b, int c, ChanB (&k)[V], float (&ga)[V]) {
+    float mean[V], rstd[V], o[V], bt[V];
+    group_pairs<V>(p.mr + (size_t)b * p.q.G * 2, p.q.cg, c, mean, rstd);
+    affine_vec<V>(p, b, c, ga, o, bt);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        k[j].mean = mean[j];
+        k[j].rstd = rstd[j];
+        k[j].mul = ga[j] * rstd[j];
+        k[j].add = o[j];
+        k[j].tol = 1e-5f * (fabsf(bt[j]) + fabsf(o[j] - bt[j]));
+        if constexpr (ACT == ACT_SILU) {
+            k[j].mul *= SILU_PRE;
+            k[j].add *= SILU_PRE;
+        }
+    }
 }
 // ReLU's gate within rounding distance of zero: the sign of u in fp64 from the unrounded factors.  u in fp32 is off by a few ulps of its
 // terms (near zero they are as large as |beta (1 + scale)| + |shift|); a gate opened by that error would change the gradient by a whole dy.  (One value in 10^5 comes here.)
@@ -311,14 +603,19 @@ __device__ __noinline__ float relu_gate64(const float* gamma, const float* beta,
     }
     return ((double)x - (double)mean) * (double)rstd * a + o > 0.0 ? 1.f : 0.f;
 }
-template <int ACT> __device__ __forceinline__ float du_of(const BwdP& p, const ChanB& k, int b, int c, float x, float dy) {
+// xc = x - mean
+template <typename T, int ACT> __device__ __forceinline__ float du_of(const BwdP& p, const ChanB& k, int b, int c, float x, float xc, float dy) {
     if constexpr (ACT == ACT_NONE) return dy;
-    const float u = fmaf(x - k.mean, k.mul, k.add);
+    const float u = fmaf(xc, k.mul, k.add);
     if constexpr (ACT == ACT_RELU) {
         if (fabsf(u) <= k.tol) return dy * relu_gate64(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, p.q.C, c, x, k.mean, k.rstd);
         return u > 0.f ? dy : 0.f * dy;
+    } else if constexpr (ACT == ACT_SILU) {  // s (1 + v (1 - s)) for v = -ln 2 u, s = 1 / (1 + 2^u)
+        const float sg = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u));
+        return dy * (sg * fmaf(u, fmaf(sg, 0.69314718055994531f, -0.69314718055994531f), 1.f));
+    } else {
+        return dy * act_slope<T, ACT>(u);
     }
-    return dy * act_d<ACT>(u);
 }
 
 // ---- pass 1: per-channel sums of du and du xhat over the rows of a split
@@ -334,25 +631,22 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_b
     const int row0 = s * q.RS, row1 = min(q.P, row0 + q.RS);
     if (ty < q.R && c < q.C) {
         ChanB k[V];
-        float s1[V], s2[V];
+        float s1[V], s2[V], ga[V];
+        chan_b<ACT, V>(p, b, c, k, ga);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            k[j] = chan_b(p, b, c + j);
-            s1[j] = s2[j] = 0.f;
-        }
-        const T* x = (const T*)p.x + (size_t)b * p.x_bs + c;
-        const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + c;
-        for (int r = row0 + ty; r < row1; r += q.R) {
-            float f[V], h[V];
-            vload<T, V>(f, x + (size_t)r * p.x_ld);
-            vload<T, V>(h, dy + (size_t)r * p.d_ld);
+        for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+        const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
+        const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + (size_t)(row0 + ty) * p.d_ld + c;
+        each_row2<4, T, V>(x, (size_t)q.R * p.x_ld, dy, (size_t)q.R * p.d_ld, rows_of(row1 - row0, ty, q.R), [&](const Raw<T, V>& vx, const Raw<T, V>& vd, int) {
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float du = du_of<ACT>(p, k[j], b, c + j, f[j], h[j]);
+                const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
                 s1[j] += du;
-                s2[j] = fmaf(du, (f[j] - k[j].mean) * k[j].rstd, s2[j]);
+                s2[j] = fmaf(du, xc, s2[j]);
             }
-        }
+        });
+#pragma unroll
+        for (int j = 0; j < V; j++) s2[j] *= k[j].rstd;
 #pragma unroll
         for (int j = 0; j < V; j++) {
             sm1[ty * q.CH + tx * V + j] = s1[j];
@@ -360,57 +654,301 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_b
         }
     }
     __syncthreads();
+    // rows of the block, per channel; then gamma' S over the channels of each group in the chunk (gamma' S rounded to fp32 as dx_of
+    // rounds gamma' du: with one value in a group both are the same number)
     for (int i = tid; i < q.CH && c0 + i < q.C; i += NT) {
         double a = 0.0, d = 0.0;
         for (int y = 0; y < q.R; y++) {
             a += (double)sm1[y * q.CH + i];
             d += (double)sm2[y * q.CH + i];
         }
+        const float s1 = (float)a, s2 = (float)d;
         float* o = p.part + (((size_t)b * q.S + s) * q.C + c0 + i) * 2;
-        o[0] = (float)a;
-        o[1] = (float)d;
+        o[0] = s1;
+        o[1] = s2;
+        float ga, be, sc;
+        affine_of(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, q.C, c0 + i, ga, be, sc);
+        sm1[i] = ga * s1;  // row 0 of its own column
+        sm2[i] = ga * s2;
     }
-}
-
-// ---- pass 2a: a thread per (image, channel): S1, S2 over the splits, the gradients of scale and shift
-__global__ __launch_bounds__(NT) void gn_bwd_chan_kernel(BwdP p) {
-    const long long i = (long long)blockIdx.x * NT + threadIdx.x;
-    const Geo& q = p.q;
-    if (i >= (long long)p.B * q.C) return;
-    const int b = (int)(i / q.C), c = (int)(i - (long long)b * q.C);
-    double a = 0.0, d = 0.0;
-    for (int s = 0; s < q.S; s++) {
-        const float* o = p.part + (((size_t)b * q.S + s) * q.C + c) * 2;
-        a += (double)o[0];
-        d += (double)o[1];
-    }
-    const float s1 = (float)a, s2 = (float)d;
-    if (p.ss) {
-        float* o = p.dss + (size_t)b * 2 * q.C;
-        o[c] = fmaf(p.gamma[c], s2, p.beta[c] * s1);
-        o[q.C + c] = s1;
-    }
-    p.sums[2 * i] = s1;
-    p.sums[2 * i + 1] = s2;
-}
-
-// ---- pass 2b: waves 0 .. B G - 1: group means m1, m2; then a wave per 64 channels: dgamma, dbeta over the images
-__global__ __launch_bounds__(NT) void gn_bwd_join_kernel(BwdP p) {
-    const Geo& q = p.q;
-    const long long w = (long long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6), ng = (long long)p.B * q.G;
-    const int lane = threadIdx.x & 63;
-    if (w < ng) {
-        const int b = (int)(w / q.G), g = (int)(w - (long long)b * q.G);
+    __syncthreads();
+    const int c1 = min(q.C, c0 + q.CH), g0 = c0 / q.cg, g1 = (c1 - 1) / q.cg, lane = tid & 63;
+    for (int g = g0 + (tid >> 6); g <= g1; g += NT / 64) {
+        const int lo = max(c0, g * q.cg) - c0, hi = min(c1, (g + 1) * q.cg) - c0;
         double a = 0.0, d = 0.0;
-        for (int e = lane; e < q.cg; e += 64) {
-            const int c = g * q.cg + e;
-            const float* o = p.sums + ((size_t)b * q.C + c) * 2;
-            // gamma' and gamma' S rounded to fp32 as dx_of rounds gamma' du: with one value in a group both are the same number
-            const float ga = p.ss ? p.gamma[c] * (1.f + p.ss[(size_t)b * p.ss_ld + p.ss_off + c]) : p.gamma[c];
-            float g1 = ga * o[0], g2 = ga * o[1];
-            asm volatile("" : "+v"(g1), "+v"(g2));
-            a += (double)g1;
-            d += (double)g2;
+        for (int e = lo + lane; e < hi; e += 64) {
+            a += (double)sm1[e];
+            d += (double)sm2[e];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            a += __shfl_xor(a, o, 64);
+            d += __shfl_xor(d, o, 64);
+        }
+        if (lane == 0) {
+            float* o = p.gpart + (((size_t)b * q.G + g) * (q.nch * q.S) + ch * q.S + s) * 2;
+            o[0] = (float)a;
+            o[1] = (float)d;
+        }
+    }
+}
+
+// group means m1, m2 from the chunks and splits, one wave
+__device__ __forceinline__ void gn_bwd_join(const BwdP& p, int b, int g, int lane, float& m1, float& m2) {
+    const Geo& q = p.q;
+    const int E = q.nch * q.S, ch0 = g * q.cg / q.CH, ch1 = ((g + 1) * q.cg - 1) / q.CH;  // other chunks hold nothing of the group
+    const float* src = p.gpart + ((size_t)b * q.G + g) * E * 2;
+    double a = 0.0, d = 0.0;
+    for (int e = ch0 * q.S + lane; e < (ch1 + 1) * q.S; e += 64) {
+        a += (double)src[2 * e];
+        d += (double)src[2 * e + 1];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        a += __shfl_xor(a, o, 64);
+        d += __shfl_xor(d, o, 64);
+    }
+    const double n = (double)q.P * (double)q.cg;
+    m1 = (float)(a / n);
+    m2 = (float)(d / n);
+}
+
+__global__ __launch_bounds__(NT) void gn_bwd_join_kernel(BwdP p, long long n) {
+    const long long i = (long long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    if (i >= n) return;
+    const int b = (int)(i / p.q.G), g = (int)(i - (long long)b * p.q.G), lane = threadIdx.x & 63;
+    float m1, m2;
+    gn_bwd_join(p, b, g, lane, m1, m2);
+    if (lane == 0) {
+        p.gm[2 * i] = m1;
+        p.gm[2 * i + 1] = m2;
+    }
+}
+
+// S1, S2 over the splits, their gradients of scale / shift, and over the images dgamma, dbeta: a block takes 8 channels, a wave
+// every fourth image, 8 lanes share the splits of a channel
+__device__ void gn_bwd_params(const BwdP& p, int blk, double (*sm)[8][2]) {
+    const Geo& q = p.q;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = blk * 8 + (lane & 7), si = lane >> 3;
+    double ga = 0.0, gb = 0.0;
+    for (int b = wave; b < p.B; b += NT / 64) {
+        double a = 0.0, d = 0.0;
+        if (c < q.C) {
+            const float* o = p.part + ((size_t)b * q.S * q.C + c) * 2;
+#pragma unroll 8
+            for (int s = si; s < q.S; s += 8) {
+                const f32x2 v = *reinterpret_cast<const f32x2*>(o + (size_t)s * q.C * 2);
+                a += (double)v[0];
+                d += (double)v[1];
+            }
+        }
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) {
+            a += __shfl_xor(a, o, 64);
+            d += __shfl_xor(d, o, 64);
+        }
+        const double s1 = (double)(float)a, s2 = (double)(float)d;
+        double sc = 1.0;
+        if (c < q.C && p.ss) {
+            sc = 1.0 + (double)p.ss[(size_t)b * p.ss_ld + p.ss_off + c];
+            if (si == 0 && p.dss) {
+                float* o = p.dss + (size_t)b * 2 * q.C;
+                o[c] = (float)((double)p.gamma[c] * s2 + (double)p.beta[c] * s1);
+                o[q.C + c] = (float)s1;
+            }
+        }
+        gb += sc * s1;
+        ga += sc * s2;
+    }
+    if (si == 0) {
+        sm[wave][lane & 7][0] = ga;
+        sm[wave][lane & 7][1] = gb;
+    }
+    __syncthreads();
+    if (tid < 8 && c < q.C) {
+        for (int w = 1; w < NT / 64; w++) {
+            ga += sm[w][tid][0];
+            gb += sm[w][tid][1];
+        }
+        p.dgamma[c] = (float)ga;
+        p.dbeta[c] = (float)gb;
+    }
+}
+
+// rstd (g - m1 - xhat m2) with rm2 = rstd m2, xc = x - mean: the product g = gamma' du is made opaque, so that the compiler does not fuse it
+// into the difference - with one value in a group, g and m1 are equal numbers and the difference has to be zero.
+__device__ __forceinline__ float dx_of(float ga, float du, float rstd, float xc, float m1, float rm2) {
+    float g = ga * du;
+    asm volatile("" : "+v"(g));
+    return rstd * ((g - m1) - xc * rm2);
+}
+
+// ---- pass 2: the first nparam blocks finish the parameters' gradients, the others write dx; every block joins its groups itself
+// (order and ONCE as in gn_apply_kernel)
+template <typename T, int V, int ACT, bool ONCE> __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(BwdP p, int nparam, int S2, int RS2, int join) {
+    __shared__ double sm_p[NT / 64][8][2];
+    __shared__ float sm_m[2 * JOIN_GROUPS];
+    if ((int)blockIdx.x < nparam) return gn_bwd_params(p, blockIdx.x, sm_p);
+    const Geo q = p.q;
+    int id = gridDim.x - 1 - blockIdx.x;
+    const int s = id % S2;
+    id /= S2;
+    const int ch = id % q.nch, b = id / q.nch;
+    const int tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
+    const int c0 = ch * q.CH, c = c0 + tx * V, g0 = c0 / q.cg, g1 = (min(q.C, c0 + q.CH) - 1) / q.cg, lane = tid & 63;
+    if (join) {
+        for (int g = g0 + (tid >> 6); g <= g1; g += NT / 64) {
+            float m1, m2;
+            gn_bwd_join(p, b, g, lane, m1, m2);
+            if (lane == 0) {
+                sm_m[2 * (g - g0)] = m1;
+                sm_m[2 * (g - g0) + 1] = m2;
+            }
+        }
+        __syncthreads();
+    }
+    if (ty >= q.R || c >= q.C) return;
+    const int row0 = s * RS2, row1 = min(q.P, row0 + RS2);
+    ChanB k[V];
+    float ga[V], m1[V], m2[V];
+    chan_b<ACT, V>(p, b, c, k, ga);
+    if (join) group_pairs<V>(sm_m - 2 * g0, q.cg, c, m1, m2);
+    else group_pairs<V>(p.gm + (size_t)b * q.G * 2, q.cg, c, m1, m2);
+#pragma unroll
+    for (int j = 0; j < V; j++) m2[j] *= k[j].rstd;
+    const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
+    const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + (size_t)(row0 + ty) * p.d_ld + c;
+    T* dx = (T*)p.dx + ((size_t)b * q.P + row0 + ty) * q.C + c;
+    const size_t ostep = (size_t)q.R * q.C;
+    each_row2<2, T, V, ONCE>(x, (size_t)q.R * p.x_ld, dy, (size_t)q.R * p.d_ld, rows_of(row1 - row0, ty, q.R), [&](const Raw<T, V>& vx, const Raw<T, V>& vd, int) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
+            o[j] = dx_of(ga[j], du, k[j].rstd, xc, m1[j], m2[j]);
+        }
+        ONCE ? vstore_once<T, V>(o, dx) : vstore<T, V>(o, dx);
+        dx += ostep;
+    });
+}
+
+// ---- one block per image and groups: S1, S2 of its channels, then dx.  IPT > 0: x and dy of all pixels stay in registers (IPT vectors per
+// thread); IPT = 0: they are read a second time (from the cache that holds them: a block's slab is at most SLAB_MAX).
+template <typename T, int ACT, int IPT, int NB> __global__ __launch_bounds__(NB) void gn_bwd_block_kernel(BwdP p, BGeo q) {
+    __shared__ float sm1[NB * 8], sm2[NB * 8];
+    __shared__ float sm_m[2 * BT];
+    const int id = xcd_run(blockIdx.x, gridDim.x), b = id / q.nch, ch = id - b * q.nch, tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
+    const int g0 = ch * q.gpc, ng = min(q.gpc, q.G - g0), c0 = g0 * q.cg, CH = ng * q.cg, c = c0 + tx * 8;
+    const bool on = ty < q.R && tx * 8 < CH;
+    constexpr int NF = IPT > 0 ? IPT : 1;
+    Raw<T, 8> fx[NF], fd[NF];
+    const int n = on ? rows_of(q.P, ty, q.R) : 0;
+    const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)ty * p.x_ld + c;
+    const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + (size_t)ty * p.d_ld + c;
+    const size_t xstep = (size_t)q.R * p.x_ld, dstep = (size_t)q.R * p.d_ld;
+    ChanB k[8];
+    float ga[8];
+    if (on) {
+        if constexpr (IPT > 0) {
+#pragma unroll
+            for (int i = 0; i < IPT; i++)
+                if (i < n) {
+                    fx[i].load(x + i * xstep);
+                    fd[i].load(dy + i * dstep);
+                }
+        }
+        float s1[8], s2[8];
+        chan_b<ACT, 8>(p, b, c, k, ga);
+#pragma unroll
+        for (int j = 0; j < 8; j++) s1[j] = s2[j] = 0.f;
+        auto sums = [&](const Raw<T, 8>& vx, const Raw<T, 8>& vd, int) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
+                s1[j] += du;
+                s2[j] = fmaf(du, xc, s2[j]);
+            }
+        };
+        if constexpr (IPT > 0) {
+#pragma unroll
+            for (int i = 0; i < IPT; i++)
+                if (i < n) sums(fx[i], fd[i], i);
+        } else {
+            each_row2<4, T, 8>(x, xstep, dy, dstep, n, sums);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) s2[j] *= k[j].rstd;
+        const int pitch = q.LP * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            sm1[ty * pitch + tx * 8 + j] = s1[j];
+            sm2[ty * pitch + tx * 8 + j] = s2[j];
+        }
+    }
+    __syncthreads();
+    {   // rows: NB / CH threads per channel add every (NB / CH)-th row, then one of them joins
+        const int pitch = q.LP * 8, ways = max(1, NB / CH), i = tid % CH, y0 = tid / CH;
+        double a = 0.0, d = 0.0;
+        if (ways > 1) {
+            if (y0 < ways)
+                for (int y = y0; y < q.R; y += ways) {
+                    a += (double)sm1[y * pitch + i];
+                    d += (double)sm2[y * pitch + i];
+                }
+            __syncthreads();
+            if (y0 < ways && y0 < q.R) {
+                sm1[y0 * CH + i] = (float)a;
+                sm2[y0 * CH + i] = (float)d;
+            }
+            __syncthreads();
+            if (tid < CH) {
+                double e = 0.0, f = 0.0;
+                for (int y = 0; y < min(ways, q.R); y++) {
+                    e += (double)sm1[y * CH + tid];
+                    f += (double)sm2[y * CH + tid];
+                }
+                sm1[tid] = (float)e;
+                sm2[tid] = (float)f;
+            }
+        } else {  // a column is read and written by one thread only
+            for (int c8 = tid; c8 < CH; c8 += NB) {
+                a = d = 0.0;
+                for (int y = 0; y < q.R; y++) {
+                    a += (double)sm1[y * pitch + c8];
+                    d += (double)sm2[y * pitch + c8];
+                }
+                sm1[c8] = (float)a;
+                sm2[c8] = (float)d;
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < CH; i += NB) {
+        const float t1 = sm1[i], t2 = sm2[i];
+        float ga, be, sc;
+        affine_of(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, q.C, c0 + i, ga, be, sc);
+        if (p.ss) {
+            float* o = p.dss + (size_t)b * 2 * q.C + c0 + i;
+            o[0] = (float)((double)p.gamma[c0 + i] * (double)t2 + (double)p.beta[c0 + i] * (double)t1);
+            o[q.C] = t1;
+        }
+        if (p.B == 1) {
+            p.dgamma[c0 + i] = t2 * sc;
+            p.dbeta[c0 + i] = t1 * sc;
+        } else {
+            p.part[((size_t)b * q.C + c0 + i) * 2] = t1;
+            p.part[((size_t)b * q.C + c0 + i) * 2 + 1] = t2;
+        }
+        sm1[i] = ga * t1;  // rounded as dx_of rounds gamma' du
+        sm2[i] = ga * t2;
+    }
+    __syncthreads();
+    const int lane = tid & 63;
+    for (int g = tid >> 6; g < ng; g += NB / 64) {
+        double a = 0.0, d = 0.0;
+        for (int e = g * q.cg + lane; e < (g + 1) * q.cg; e += 64) {
+            a += (double)sm1[e];
+            d += (double)sm2[e];
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
@@ -419,111 +957,194 @@ __global__ __launch_bounds__(NT) void gn_bwd_join_kernel(BwdP p) {
         }
         const double n = (double)q.P * (double)q.cg;
         if (lane == 0) {
-            p.gm[2 * w] = (float)(a / n);
-            p.gm[2 * w + 1] = (float)(d / n);
+            sm_m[2 * g] = (float)(a / n);
+            sm_m[2 * g + 1] = (float)(d / n);
         }
+    }
+    __syncthreads();
+    if (!on) return;
+    float m1[8], m2[8];
+    group_pairs<8>(sm_m, q.cg, tx * 8, m1, m2);
+#pragma unroll
+    for (int j = 0; j < 8; j++) m2[j] *= k[j].rstd;
+    T* dx = (T*)p.dx + ((size_t)b * q.P + ty) * q.C + c;
+    const size_t ostep = (size_t)q.R * q.C;
+    auto write = [&](const Raw<T, 8>& vx, const Raw<T, 8>& vd, int) {
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
+            o[j] = dx_of(ga[j], du, k[j].rstd, xc, m1[j], m2[j]);
+        }
+        vstore<T, 8>(o, dx);
+        dx += ostep;
+    };
+    if constexpr (IPT > 0) {
+#pragma unroll
+        for (int i = 0; i < IPT; i++)
+            if (i < n) write(fx[i], fd[i], i);
     } else {
-        const long long c = (w - ng) * 64 + lane;
-        if (c >= q.C) return;
-        double a = 0.0, d = 0.0;
-        for (int b = 0; b < p.B; b++) {
-            const float* o = p.sums + ((size_t)b * q.C + c) * 2;
-            const double sc = p.ss ? 1.0 + (double)p.ss[(size_t)b * p.ss_ld + p.ss_off + c] : 1.0;
-            a += sc * (double)o[0];
-            d += sc * (double)o[1];
-        }
-        p.dbeta[c] = (float)a;
-        p.dgamma[c] = (float)d;
+        each_row2<2, T, 8>(x, xstep, dy, dstep, n, write);
     }
 }
-
-// rstd (g - m1 - xhat m2): the product g = gamma' du is made opaque, so that the compiler does not fuse it into the difference - with one
-// value in a group, g and m1 are equal numbers and the difference has to be zero.
-__device__ __forceinline__ float dx_of(float ga, float du, float rstd, float xh, float m1, float m2) {
-    float g = ga * du;
-    asm volatile("" : "+v"(g));
-    return rstd * ((g - m1) - xh * m2);
-}
-
-// ---- pass 3: dx
-template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(BwdP p) {
-    const Geo q = p.q;
-    int id = blockIdx.x;
-    const int s = id % q.S;
-    id /= q.S;
-    const int ch = id % q.nch, b = id / q.nch;
-    const int tid = threadIdx.x, tx = tid % q.LP, ty = tid / q.LP;
-    const int c = ch * q.CH + tx * V;
-    if (ty >= q.R || c >= q.C) return;
-    const int row0 = s * q.RS, row1 = min(q.P, row0 + q.RS);
-    ChanB k[V];
-    float ga[V], m1[V], m2[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        k[j] = chan_b(p, b, c + j);
-        float o, sc;
-        affine_of(p.gamma, p.beta, p.ss, p.ss_ld, p.ss_off, b, q.C, c + j, ga[j], o, sc);
-        const float* gm = p.gm + ((size_t)b * q.G + (c + j) / q.cg) * 2;
-        m1[j] = gm[0];
-        m2[j] = gm[1];
-    }
-    const T* x = (const T*)p.x + (size_t)b * p.x_bs + c;
-    const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + c;
-    T* dx = (T*)p.dx + (size_t)b * q.P * q.C + c;
-    for (int r = row0 + ty; r < row1; r += q.R) {
-        float f[V], h[V];
-        vload<T, V>(f, x + (size_t)r * p.x_ld);
-        vload<T, V>(h, dy + (size_t)r * p.d_ld);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const float du = du_of<ACT>(p, k[j], b, c + j, f[j], h[j]);
-            f[j] = dx_of(ga[j], du, k[j].rstd, (f[j] - k[j].mean) * k[j].rstd, m1[j], m2[j]);
-        }
-        vstore<T, V>(f, dx + (size_t)r * q.C);
-    }
+__global__ __launch_bounds__(NT) void gn_bwd_params_kernel(BwdP p) {
+    __shared__ double sm[NT / 64][8][2];
+    gn_bwd_params(p, blockIdx.x, sm);
 }
 
 // ================================================== host ==================================================
-constexpr int ROWS_PER_THREAD = 32;
+constexpr int ROWS_PER_THREAD = 8;
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+int wide_params(const float* gamma, const float* beta, const float* ss, int ss_ld, int ss_off, int C) {
+    return aligned16(gamma) && aligned16(beta) && (!ss || (aligned16(ss) && ss_ld % 4 == 0 && ss_off % 4 == 0 && C % 4 == 0));
+}
+
 Geo geo_any(int P, int C, int G, bool vec) { return geo_of(P, C, G, vec ? 8 : 1, ROWS_PER_THREAD); }
 
-template <typename T, int V> int fwd_launch(const FwdP& p, int B, int act, hipStream_t st) {
-    const Geo& q = p.q;
-    const dim3 grid((unsigned)(B * q.nch * q.S));
-    hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(NT), 0, st, p);
-    const long long n = (long long)B * q.G;
-    hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);
-    switch (act) {
-        case ACT_RELU: hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_RELU>), grid, dim3(NT), 0, st, p); break;
-        case ACT_GELU: hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_GELU>), grid, dim3(NT), 0, st, p); break;
-        case ACT_SILU: hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_SILU>), grid, dim3(NT), 0, st, p); break;
-        default: hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_NONE>), grid, dim3(NT), 0, st, p); break;
-    }
+// Rows of a pass that needs no fixed split: about 2048 blocks in all, at least 4 rows per thread
+void apply_split(const Geo& q, int B, int& S2, int& RS2) {
+    long long want = 2048 / ((long long)B * q.nch);
+    const long long most = (q.P + 4ll * q.R - 1) / (4ll * q.R);
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    RS2 = (int)((q.P + want - 1) / want);
+    S2 = (q.P + RS2 - 1) / RS2;
+}
+
+// The one-block form: as few whole groups per block as make 64-byte rows of whole vectors.  Returns the vectors per thread, 0 if the shape has none.
+int block_geo(int P, int C, int G, int esize, BGeo& q) {
+    const int cg = C / G;
+    int gpc = 1;
+    while (gpc < G && ((gpc * cg) % 8 != 0 || gpc * cg * esize < 64)) gpc++;
+    if ((gpc * cg) % 8 != 0 || gpc * cg / 8 > BT || gpc > BT) return 0;
+    q.P = P;
+    q.C = C;
+    q.G = G;
+    q.cg = cg;
+    q.gpc = gpc;
+    q.nch = (G + gpc - 1) / gpc;
+    q.LP = gpc * cg / 8;
+    q.R = BT / q.LP;
+    const long long n = ((long long)P + q.R - 1) / q.R;
+    return n > (1 << 20) ? (1 << 20) : (int)n;
+}
+// whether every block of the last pass joins the groups of its chunk itself: few groups with few partials (a wave's round trip each)
+bool joins_in_block(const Geo& q) {
+    int groups = (q.CH + q.cg - 1) / q.cg + 1;  // that meet a chunk, at most
+    if (groups > q.G) groups = q.G;
+    return groups <= JOIN_GROUPS && (long long)groups * q.nch * q.S <= JOIN_MAX;
+}
+bool read_once(long long bytes) { return bytes > (128ll << 20); }
+constexpr int SLAB_BT = 512;
+constexpr int SLAB_MAX = 512 << 10;  // bytes of x that one block of the backward reads twice
+
+template <typename T, int ACT> int fwd_launch_vec(const FwdP& p, int B, hipStream_t st, bool& done) {
+    BGeo g;
+    const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
+    done = n > 0 && n <= (sizeof(T) == 2 ? 32 : 16);
+    if (!done) return DIG_OK;
+    DIG_CHECK((long long)B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
+    const dim3 grid((unsigned)(B * g.nch));
+    if (n <= 2) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 2>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= 4) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 4>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= 8) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 8>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= 16) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 16>), grid, dim3(BT), 0, st, p, g);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 32>), grid, dim3(BT), 0, st, p, g);
     DIG_LAUNCH_CHECK("gn_act");
     return DIG_OK;
 }
 
-template <typename T, int V, int ACT> void bwd_launch_act(const BwdP& p, hipStream_t st) {
+template <typename T, int V, int ACT> int fwd_launch(const FwdP& p, int B, hipStream_t st) {
+    if constexpr (V == 8) {
+        bool done;
+        const int rc = fwd_launch_vec<T, ACT>(p, B, st, done);
+        if (done) return rc;
+    }
     const Geo& q = p.q;
-    const dim3 grid((unsigned)(p.B * q.nch * q.S));
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT>), grid, dim3(NT), 0, st, p);
-    const long long bc = (long long)p.B * q.C, waves = (long long)p.B * q.G + (q.C + 63) / 64;
-    hipLaunchKernelGGL(gn_bwd_chan_kernel, dim3((unsigned)((bc + NT - 1) / NT)), dim3(NT), 0, st, p);
-    hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)((waves + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p);
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT>), grid, dim3(NT), 0, st, p);
+    const int join = joins_in_block(q);
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)(B * q.nch * q.S)), dim3(NT), 0, st, p);
+    if (!join) {
+        const long long n = (long long)B * q.G;
+        hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);
+    }
+    int S2, RS2;
+    apply_split(q, B, S2, RS2);
+    const dim3 grid((unsigned)(B * q.nch * S2));
+    if (V == 8 && read_once((long long)B * q.P * q.C * (long long)sizeof(T)))
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true>), grid, dim3(NT), 0, st, p, S2, RS2, join);
+    else hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false>), grid, dim3(NT), 0, st, p, S2, RS2, join);
+    DIG_LAUNCH_CHECK("gn_act");
+    return DIG_OK;
 }
-template <typename T, int V> int bwd_launch(const BwdP& p, int act, hipStream_t st) {
+template <typename T, int V> int fwd_act(const FwdP& p, int B, int act, hipStream_t st) {
     switch (act) {
-        case ACT_RELU: bwd_launch_act<T, V, ACT_RELU>(p, st); break;
-        case ACT_GELU: bwd_launch_act<T, V, ACT_GELU>(p, st); break;
-        case ACT_SILU: bwd_launch_act<T, V, ACT_SILU>(p, st); break;
-        default: bwd_launch_act<T, V, ACT_NONE>(p, st); break;
+        case ACT_RELU: return fwd_launch<T, V, ACT_RELU>(p, B, st);
+        case ACT_GELU: return fwd_launch<T, V, ACT_GELU>(p, B, st);
+        case ACT_SILU: return fwd_launch<T, V, ACT_SILU>(p, B, st);
+        default: return fwd_launch<T, V, ACT_NONE>(p, B, st);
+    }
+}
+
+template <typename T, int ACT> int bwd_launch_vec(BwdP p, hipStream_t st, bool& done) {
+    BGeo g;
+    const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
+    const int most = sizeof(T) == 2 ? 16 : 8;
+    done = n > 0 && (n <= most || (long long)p.q.P * g.LP * 8 * (long long)sizeof(T) <= SLAB_MAX);
+    if (!done) return DIG_OK;
+    DIG_CHECK((long long)p.B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
+    const dim3 grid((unsigned)(p.B * g.nch));
+    if (n <= 2) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 2, BT>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= 4) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 4, BT>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= 8) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 8, BT>), grid, dim3(BT), 0, st, p, g);
+    else if (n <= most) {
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 16, BT>), grid, dim3(BT), 0, st, p, g);
+    } else {
+        g.R = SLAB_BT / g.LP;
+        hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 0, SLAB_BT>), grid, dim3(SLAB_BT), 0, st, p, g);
+    }
+    if (p.B > 1) {  // part is [B][C][2] here: the gradients of the parameters over the images
+        BwdP r = p;
+        r.q.S = 1;
+        r.dss = nullptr;  // written by the blocks
+        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)((p.q.C + 7) / 8)), dim3(NT), 0, st, r);
     }
     DIG_LAUNCH_CHECK("gn_act_bwd");
     return DIG_OK;
+}
+
+template <typename T, int V, int ACT> int bwd_launch(const BwdP& p, hipStream_t st) {
+    if constexpr (V == 8) {
+        bool done;
+        const int rc = bwd_launch_vec<T, ACT>(p, st, done);
+        if (done) return rc;
+    }
+    const Geo& q = p.q;
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT>), dim3((unsigned)(p.B * q.nch * q.S)), dim3(NT), 0, st, p);
+    const int nparam = (q.C + 7) / 8;
+    int S2, RS2;
+    apply_split(q, p.B, S2, RS2);
+    const int join = joins_in_block(q);
+    if (!join) {
+        const long long n = (long long)p.B * q.G;
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);
+    }
+    DIG_CHECK((long long)p.B * q.nch * S2 + nparam < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
+    const dim3 grid((unsigned)(p.B * q.nch * S2 + nparam));
+    if (V == 8 && read_once(2ll * p.B * q.P * q.C * (long long)sizeof(T)))
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true>), grid, dim3(NT), 0, st, p, nparam, S2, RS2, join);
+    else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false>), grid, dim3(NT), 0, st, p, nparam, S2, RS2, join);
+    DIG_LAUNCH_CHECK("gn_act_bwd");
+    return DIG_OK;
+}
+template <typename T, int V> int bwd_act(const BwdP& p, int act, hipStream_t st) {
+    switch (act) {
+        case ACT_RELU: return bwd_launch<T, V, ACT_RELU>(p, st);
+        case ACT_GELU: return bwd_launch<T, V, ACT_GELU>(p, st);
+        case ACT_SILU: return bwd_launch<T, V, ACT_SILU>(p, st);
+        default: return bwd_launch<T, V, ACT_NONE>(p, st);
+    }
 }
 
 bool shape_ok(int B, int P, int C, int G) { return B > 0 && P > 0 && C > 0 && G > 0 && C % G == 0 && P <= (1 << 30) && C <= (1 << 20); }
@@ -535,7 +1156,7 @@ extern "C" int dig_gn_act_ws(int P, int C, int groups, int bwd) {
     int most = 0;
     for (int vec = 0; vec < 2; vec++) {  // whichever of the two the strides and the alignment will select
         const Geo q = geo_any(P, C, groups, vec != 0);
-        const int n = bwd ? q.S * C * 2 + C * 2 + groups * 2 : groups * q.nch * q.S * 2;
+        const int n = (bwd ? q.S * C * 2 + groups * 2 : 0) + groups * q.nch * q.S * 2;
         most = n > most ? n : most;
     }
     return most;
@@ -550,11 +1171,11 @@ extern "C" int dig_gn_act(const dig_gn_act_args* a, void* stream) {
               a->ss_off, a->C);
     const bool vec = a->C % 8 == 0 && a->x_bs % 8 == 0 && a->x_ld % 8 == 0 && aligned16(a->x) && aligned16(a->out) &&
                      (!a->res || (a->res_bs % 8 == 0 && a->res_ld % 8 == 0 && aligned16(a->res)));
-    FwdP p{a->x, a->gamma, a->beta, a->ss, a->res, a->out, a->mean_rstd, a->ws, a->x_bs, a->x_ld, a->res_bs, a->res_ld, a->ss_ld, a->ss_off, a->eps, geo_any(a->P, a->C, a->groups, vec)};
+    FwdP p{a->x, a->gamma, a->beta, a->ss, a->res, a->out, a->mean_rstd, a->ws, a->x_bs, a->x_ld, a->res_bs, a->res_ld, a->ss_ld, a->ss_off, wide_params(a->gamma, a->beta, a->ss, a->ss_ld, a->ss_off, a->C), a->eps, geo_any(a->P, a->C, a->groups, vec)};
     DIG_CHECK((long long)a->B * p.q.nch * p.q.S < (1ll << 31) && (long long)a->B * a->groups < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == DIG_BF16) return vec ? fwd_launch<bf16, 8>(p, a->B, a->act, st) : fwd_launch<bf16, 1>(p, a->B, a->act, st);
-    return vec ? fwd_launch<float, 8>(p, a->B, a->act, st) : fwd_launch<float, 1>(p, a->B, a->act, st);
+    if (a->dtype == DIG_BF16) return vec ? fwd_act<bf16, 8>(p, a->B, a->act, st) : fwd_act<bf16, 1>(p, a->B, a->act, st);
+    return vec ? fwd_act<float, 8>(p, a->B, a->act, st) : fwd_act<float, 1>(p, a->B, a->act, st);
 }
 
 extern "C" int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream) {
@@ -568,12 +1189,12 @@ extern "C" int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream) {
                      aligned16(a->dx);
     const Geo q = geo_any(a->P, a->C, a->groups, vec);
     float* part = a->ws;
-    float* sums = part + (size_t)a->B * q.S * a->C * 2;
-    float* gm = sums + (size_t)a->B * a->C * 2;
-    BwdP p{a->x, a->dy, a->mean_rstd, a->gamma, a->beta, a->ss, a->dx, a->dgamma, a->dbeta, a->dss, part, sums, gm, a->x_bs, a->x_ld, a->dy_bs, a->dy_ld, a->ss_ld,
-           a->ss_off, a->B, q};
+    float* gpart = part + (size_t)a->B * q.S * a->C * 2;
+    float* gm = gpart + (size_t)a->B * a->groups * q.nch * q.S * 2;
+    BwdP p{a->x, a->dy, a->mean_rstd, a->gamma, a->beta, a->ss, a->dx, a->dgamma, a->dbeta, a->dss, part, gpart, gm, a->x_bs, a->x_ld, a->dy_bs, a->dy_ld, a->ss_ld,
+           a->ss_off, wide_params(a->gamma, a->beta, a->ss, a->ss_ld, a->ss_off, a->C), a->B, q};
     DIG_CHECK((long long)a->B * q.nch * q.S < (1ll << 31) && (long long)a->B * a->groups < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == DIG_BF16) return vec ? bwd_launch<bf16, 8>(p, a->act, st) : bwd_launch<bf16, 1>(p, a->act, st);
-    return vec ? bwd_launch<float, 8>(p, a->act, st) : bwd_launch<float, 1>(p, a->act, st);
+    if (a->dtype == DIG_BF16) return vec ? bwd_act<bf16, 8>(p, a->act, st) : bwd_act<bf16, 1>(p, a->act, st);
+    return vec ? bwd_act<float, 8>(p, a->act, st) : bwd_act<float, 1>(p, a->act, st);
 }
