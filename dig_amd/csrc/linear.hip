@@ -38,17 +38,20 @@ struct LinP {
     int act, out_f32, vec;  // vec: 8-column vectors of out / pre / res are 16-byte aligned
 };
 
+template <bool FULL> __device__ __forceinline__ void load_bias(const LinP& p, int c, float (&bias)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) bias[j] = FULL && p.bias && c + j < p.C ? p.bias[c + j] : 0.f;
+}
+
 // 8 columns of the epilogue from column c of row r: n of them exist.  FULL: bias, pre, act and res; otherwise only the store.  rv: the
 // residual's vector, if p.vec
-template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(const LinP& p, float (&v)[8], int r, int c, int n, const Frag<T>& rv) {
+template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(const LinP& p, float (&v)[8], int r, int c, int n, const Frag<T>& rv, const float (&bias)[8]) {
     const size_t o = (size_t)r * p.ldo + c;
     if (p.vec) {  // n is 8
         Frag<T> f;
         if constexpr (FULL) {
-            if (p.bias) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] += p.bias[c + j];
-            }
+            for (int j = 0; j < 8; j++) v[j] += bias[j];
             if (p.pre) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) frag_set<T>(f, j, v[j]);
@@ -77,7 +80,7 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(c
         if (j < n) {
             float z = v[j];
             if constexpr (FULL) {
-                if (p.bias) z += p.bias[c + j];
+                z += bias[j];
                 if (p.pre) ((T*)p.pre)[o + j] = from_f32<T>(z);
                 z = act_val<T, ACT>(z);
                 if (p.res) z += to_f32<T>(((const T*)p.res)[(size_t)r * p.ldr + c + j]);
@@ -88,8 +91,13 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(c
     }
 }
 
-typedef std::integral_constant<bool, true> yes;
-typedef std::integral_constant<bool, false> no;
+// f(0), ..., f(N - 1) with constant indices: hipcc gives up on unrolling a large body, and an array of accumulators indexed by a variable goes to memory
+template <int N, typename F> __device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>());
+    }
+}
 
 constexpr int KB = 128;  // bytes of k in a tile: 64 bf16 or 32 fp32 values
 
@@ -175,7 +183,7 @@ template <int N> __device__ __forceinline__ void dma_wait_barrier() { asm volati
 // Otherwise (TQ): two tiles in LDS, filled through registers, which fetch a tile ahead - hipcc waits for every DMA in flight before a transposing
 // read, so the two do not go together.
 template <typename T, bool TP, bool TQ, int BR, int BC, int WR, int WC, int NS, bool ALIGNED, bool FULL>
-__global__ __launch_bounds__(WR* WC * 64, BR * BC <= 128 * 128 || WR * WC == 8 ? 2 : 1) void linear_kernel(LinP p, int rtiles, int ctiles) {
+__device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctiles, int id, unsigned char* smem) {
     using SP = Side<T, TP, BR>;
     using SQ = Side<T, TQ, BC>;
     using F = typename Ops<T>::F;
@@ -189,10 +197,8 @@ __global__ __launch_bounds__(WR* WC * 64, BR * BC <= 128 * 128 || WR * WC == 8 ?
     constexpr bool STAGED = TQ;
     static_assert(!STAGED || NS == 2, "two tiles");
     static_assert(TRN >= 2, "rows to spread the reads over");
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-
     // tiles to XCDs: each of the 8 gets a contiguous run of tiles (block index modulo 8 is the XCD), so that what neighbours share stays in its L2
-    const int ntiles = rtiles * ctiles, id = blockIdx.x;
+    const int ntiles = rtiles * ctiles;
     int t = id % ntiles;
     const int split = id / ntiles;
     {
@@ -367,68 +373,74 @@ __global__ __launch_bounds__(WR* WC * 64, BR * BC <= 128 * 128 || WR * WC == 8 ?
         }
     }
 
-    // ---- epilogue: 16 rows of the wave's columns at a time through its own LDS rows, then 8 adjacent columns per lane.  The residual of
-    // the next 16 rows is fetched while these are worked on.
+    // ---- epilogue: 16 rows of the wave's columns at a time through LDS rows of its own (two sets: the next rows are written while these
+    // are worked on), then 8 adjacent columns per lane.  The residual of the next 16 rows is fetched meanwhile; a lane's columns stay the same.
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last matrix instructions have retired before their registers are read
     __syncthreads();                                     // every wave is done with the operand tiles
-    float* ot = reinterpret_cast<float*>(smem) + wave * 16 * OS;
+    float* ot = reinterpret_cast<float*>(smem) + wave * 2 * 16 * OS;
     const int i16 = lane & 15, q4 = lane >> 4;
-    constexpr int ITEMS = 16 * WCOLS / 8 / 64;
-    static_assert(ITEMS >= 1, "a wave has at least 32 columns");
+    constexpr int LPR = WCOLS / 8, ITEMS = 16 * LPR / 64, STEP = 64 / LPR;  // lanes per row; rows between a lane's items
+    static_assert(ITEMS >= 1 && 64 % LPR == 0, "a wave has 32, 64 or more columns");
     float* part = p.splits > 1 ? p.part + (size_t)split * p.R * p.C : nullptr;
     const bool use_res = FULL && p.res && p.vec && !part;
-    auto place = [&](int i, int it, int& r, int& c) {
-        const int idx = lane + it * 64;
-        r = r0 + wr * (BR / WR) + i * 16 + idx / (WCOLS / 8);
-        c = c0 + wc * WCOLS + (idx % (WCOLS / 8)) * 8;
-    };
+    const int rl = lane / LPR, cl = lane % LPR * 8, rfirst = r0 + wr * (BR / WR) + rl, c = c0 + wc * WCOLS + cl, n = min(8, p.C - c);
+    float bias[8];
+    load_bias<FULL>(p, c, bias);
     Frag<T> rn[ITEMS];
     auto fetch_res = [&](int i) {
 #pragma unroll
         for (int it = 0; it < ITEMS; it++) {
-            int r, c;
-            place(i, it, r, c);
-            if (r < p.R && c < p.C) frag_load<T>(rn[it], (const T*)p.res + (size_t)r * p.ldr + c);
+            const int r = rfirst + i * 16 + it * STEP;
+            if (r < p.R && n > 0) frag_load<T>(rn[it], (const T*)p.res + (size_t)r * p.ldr + c);
         }
+    };
+    auto put_rows = [&](auto row) {
+        constexpr int i = decltype(row)::value;
+#pragma unroll
+        for (int j = 0; j < TCN; j++) *reinterpret_cast<f32x4*>(ot + (i & 1) * 16 * OS + i16 * OS + j * 16 + q4 * 4) = acc[i][j];
     };
     auto finish = [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         if (use_res) fetch_res(0);
-#pragma unroll
-        for (int i = 0; i < TRN; i++) {
-#pragma unroll
-            for (int j = 0; j < TCN; j++) *reinterpret_cast<f32x4*>(ot + i16 * OS + j * 16 + q4 * 4) = acc[i][j];
+        put_rows(std::integral_constant<int, 0>());
+        static_for<TRN>([&](auto row) {
+            constexpr int i = decltype(row)::value;
             __builtin_amdgcn_wave_barrier();
+            f32x4 a[ITEMS], b[ITEMS];
             Frag<T> rv[ITEMS];
 #pragma unroll
-            for (int it = 0; it < ITEMS; it++) rv[it] = rn[it];
-            if (use_res && i + 1 < TRN) fetch_res(i + 1);
+            for (int it = 0; it < ITEMS; it++) {
+                const float* at = ot + (i & 1) * 16 * OS + (rl + it * STEP) * OS + cl;
+                a[it] = *reinterpret_cast<const f32x4*>(at);
+                b[it] = *reinterpret_cast<const f32x4*>(at + 4);
+                rv[it] = rn[it];
+            }
+            if constexpr (i + 1 < TRN) {
+                put_rows(std::integral_constant<int, i + 1>());
+                if (use_res) fetch_res(i + 1);
+            }
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int it = 0; it < ITEMS; it++) {
-                const int idx = lane + it * 64, rl = idx / (WCOLS / 8), cl = (idx % (WCOLS / 8)) * 8;
-                int r, c;
-                place(i, it, r, c);
-                const f32x4 a = *reinterpret_cast<const f32x4*>(ot + rl * OS + cl), b = *reinterpret_cast<const f32x4*>(ot + rl * OS + cl + 4);
-                if (r < p.R && c < p.C) {
-                    const int n = min(8, p.C - c);
-                    float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                const int r = rfirst + i * 16 + it * STEP;
+                if (r < p.R && n > 0) {
+                    float v[8] = {a[it][0], a[it][1], a[it][2], a[it][3], b[it][0], b[it][1], b[it][2], b[it][3]};
                     if (part) {
                         float* d = part + (size_t)r * p.C + c;
                         if (n == 8 && p.C % 4 == 0) {
-                            *reinterpret_cast<f32x4*>(d) = a;
-                            *reinterpret_cast<f32x4*>(d + 4) = b;
+                            *reinterpret_cast<f32x4*>(d) = a[it];
+                            *reinterpret_cast<f32x4*>(d + 4) = b[it];
                         } else {
 #pragma unroll
                             for (int e = 0; e < 8; e++)
                                 if (e < n) d[e] = v[e];
                         }
                     } else {
-                        epi8<T, ACT, FULL>(p, v, r, c, n, rv[it]);
+                        epi8<T, ACT, FULL>(p, v, r, c, n, rv[it], bias);
                     }
                 }
             }
-            __builtin_amdgcn_wave_barrier();
-        }
+        });
     };
     if constexpr (FULL) {
         if (p.act == ACT_RELU) finish(std::integral_constant<int, ACT_RELU>());
@@ -440,18 +452,26 @@ __global__ __launch_bounds__(WR* WC * 64, BR * BC <= 128 * 128 || WR * WC == 8 ?
     }
 }
 
+// MINW waves per SIMD: it bounds the registers, and with at most 256 of them hipcc keeps the accumulators where the matrix instructions read them (with
+// more it moves them between the two register files in every K step)
+template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW, bool ALIGNED> __global__ __launch_bounds__(WR* WC * 64, MINW) void linear_kernel(LinP p, int rtiles, int ctiles) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    linear_tile<T, false, false, BR, BC, WR, WC, NS, ALIGNED, true>(p, rtiles, ctiles, blockIdx.x, smem);
+}
+
 // splits > 1: the partial products of a row's 8 columns, added in order, and the epilogue
-template <typename T, int ACT, bool FULL> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) {
+template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear_join(const LinP& p, int blk) {
     const int cv = (p.C + 7) / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = (long long)blk * 256 + threadIdx.x;
     if (i >= (long long)p.R * cv) return;
     const int r = (int)(i / cv), c = (int)(i - (long long)r * cv) * 8, n = min(8, p.C - c);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const float* s = p.part + (size_t)r * p.C + c;
     const size_t step = (size_t)p.R * p.C;
     if (n == 8 && p.C % 4 == 0) {
-        for (int k = 0; k < p.splits; k++, s += step) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(s), b = *reinterpret_cast<const f32x4*>(s + 4);
+#pragma unroll 4
+        for (int k = 0; k < p.splits; k++) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(s + k * step), b = *reinterpret_cast<const f32x4*>(s + k * step + 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 v[e] += a[e];
@@ -459,15 +479,18 @@ template <typename T, int ACT, bool FULL> __global__ __launch_bounds__(256) void
             }
         }
     } else {
-        for (int k = 0; k < p.splits; k++, s += step)
+        for (int k = 0; k < p.splits; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (e < n) v[e] += s[e];
+                if (e < n) v[e] += s[k * step + e];
     }
     Frag<T> rv;
     if (FULL && p.res && p.vec) frag_load<T>(rv, (const T*)p.res + (size_t)r * p.ldr + c);
-    epi8<T, ACT, FULL>(p, v, r, c, n, rv);
+    float bias[8];
+    load_bias<FULL>(p, c, bias);
+    epi8<T, ACT, FULL>(p, v, r, c, n, rv, bias);
 }
+template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) { linear_join<T, ACT, true>(p, blockIdx.x); }
 
 // ---- dz = dy act'(z), and the column sums of the unrounded dz: a block takes 256 V columns by RPB rows
 struct DzP {
@@ -477,10 +500,9 @@ struct DzP {
     float* part;    // [row blocks][N], or NULL
     int M, N, ldz, rows;
 };
-template <typename T, int V, int ACT> __global__ __launch_bounds__(256) void linear_dz_kernel(DzP p) {
-    const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * V, ty = threadIdx.x >> 6;
-    const int row0 = blockIdx.y * p.rows, row1 = min(p.M, row0 + p.rows), width = p.dz ? p.ldz : p.N;
-    __shared__ float sm[4][64 * V + 1];
+template <typename T, int V, int ACT> __device__ __forceinline__ void linear_dz(const DzP& p, int bx, int by, float* sm) {  // sm: 4 rows of 64 V + 1
+    const int c = (bx * 64 + (threadIdx.x & 63)) * V, ty = threadIdx.x >> 6;
+    const int row0 = by * p.rows, row1 = min(p.M, row0 + p.rows), width = p.dz ? p.ldz : p.N;
     float s[V];
 #pragma unroll
     for (int j = 0; j < V; j++) s[j] = 0.f;
@@ -516,17 +538,22 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(256) void lin
     }
     if (!p.part) return;
 #pragma unroll
-    for (int j = 0; j < V; j++) sm[ty][(threadIdx.x & 63) * V + j] = s[j];
+    for (int j = 0; j < V; j++) sm[ty * (64 * V + 1) + (threadIdx.x & 63) * V + j] = s[j];
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * V; i += 256) {
-        const int col = blockIdx.x * 64 * V + i;
-        if (col < p.N) p.part[(size_t)blockIdx.y * p.N + col] = (sm[0][i] + sm[1][i]) + (sm[2][i] + sm[3][i]);
+        const int col = bx * 64 * V + i;
+        constexpr int W = 64 * V + 1;
+        if (col < p.N) p.part[(size_t)by * p.N + col] = (sm[i] + sm[W + i]) + (sm[2 * W + i] + sm[3 * W + i]);
     }
 }
-__global__ __launch_bounds__(256) void linear_db_kernel(const float* part, float* db, int chunks, int N) {
+template <typename T, int V, int ACT> __global__ __launch_bounds__(256) void linear_dz_kernel(DzP p) {
+    __shared__ float sm[4 * (64 * V + 1)];
+    linear_dz<T, V, ACT>(p, blockIdx.x, blockIdx.y, sm);
+}
+__device__ __forceinline__ void linear_db(const float* part, float* db, int chunks, int N, int blk) {
     // 16 lanes x 16 columns: 16 strides of the chunks, joined in LDS in fp64
     __shared__ double sm[16][17];
-    const int cx = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + cx;
+    const int cx = threadIdx.x & 15, y = threadIdx.x >> 4, c = blk * 16 + cx;
     double s = 0.0;
     if (c < N)
         for (int k = y; k < chunks; k += 16) s += (double)part[(size_t)k * N + c];
@@ -538,102 +565,104 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, float
     }
 }
 
+// ---- the products of the backward in one launch: the blocks of dW, those of dx and, without an activation, those of the column sums of dy.
+// Two 128 x 128 blocks per CU; one launch fills the chip where dW (few tiles, long k) or dx alone would not, and the tails overlap.
+struct BwdP {
+    LinP w, x;
+    int wr, wc, xr, xc;           // tiles
+    int n0, n1;                   // blocks of the first and of the first two segments (multiples of 8, so that block index modulo 8 stays the XCD)
+    int w_first;                  // the segment with the longer blocks comes first
+    DzP s;
+    int sx;                       // column blocks of the sums
+};
+template <typename T, bool ALIGNED, int SV> __global__ __launch_bounds__(256, 2) void linear_bwd_kernel(BwdP p) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    const int id = blockIdx.x;
+    if (id >= p.n1) {
+        if constexpr (SV > 0) linear_dz<T, SV, ACT_NONE>(p.s, (id - p.n1) % p.sx, (id - p.n1) / p.sx, reinterpret_cast<float*>(smem));
+        return;
+    }
+    const bool first = id < p.n0;
+    const int at = first ? id : id - p.n0;
+    if (first == (p.w_first != 0)) {
+        if (at < p.wr * p.wc * p.w.splits) linear_tile<T, true, true, 128, 128, 2, 2, 2, ALIGNED, false>(p.w, p.wr, p.wc, at, smem);
+    } else {
+        if (at < p.xr * p.xc * p.x.splits) linear_tile<T, false, true, 128, 128, 2, 2, 2, ALIGNED, false>(p.x, p.xr, p.xc, at, smem);
+    }
+}
+// what remains: the joins of dW and dx, and db from the column sums
+template <typename T> __global__ __launch_bounds__(256) void linear_bwd_join_kernel(LinP w, LinP x, int nw, int nx, const float* sums, float* db, int chunks, int N) {
+    const int id = blockIdx.x;
+    if (id < nw) linear_join<T, ACT_NONE, false>(w, id);
+    else if (id < nw + nx) linear_join<T, ACT_NONE, false>(x, id - nw);
+    else linear_db(sums, db, chunks, N, id - nw - nx);
+}
+
 // ================================================== host ==================================================
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr int TILE = 128;
-#ifndef BIG_TILE
-#define BIG_TILE 0
-#define BT_R 256
-#define BT_C 256
-#define BT_WR 2
-#define BT_WC 2
-#define BT_NS 2
-#endif
+inline int up(int a, int b) { return (a + b - 1) / b; }
 
-// k slices of a product whose tiles do not fill the chip: about two blocks per CU, at least 4 k tiles per slice
-void split_of(int R, int C, int K, int bk, int& splits, int& kper) {
-    const long long tiles = (long long)((R + TILE - 1) / TILE) * ((C + TILE - 1) / TILE);
-    const int nk = (K + bk - 1) / bk;
-    int s = tiles >= 256 ? 1 : (int)(512 / tiles);
-    if (s > nk / 4) s = nk / 4;
-    if (s < 1) s = 1;
-    const int per = (nk + s - 1) / s;
-    splits = (nk + per - 1) / per;
-    if (splits < 1) splits = 1;
-    kper = per * bk;
+void set_split(LinP& p, int s, int bk) {
+    const int nk = up(p.K, bk), per = up(nk, s);
+    p.splits = up(nk, per);
+    p.kper = per * bk;
 }
 
-template <typename T, bool FULL> void join_launch(const LinP& p, hipStream_t st) {
-    const long long n = (long long)p.R * ((p.C + 7) / 8);
-    const dim3 grid((unsigned)((n + 255) / 256));
-    if constexpr (FULL) {
-        switch (p.act) {
-            case ACT_RELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_RELU, true>), grid, dim3(256), 0, st, p); return;
-            case ACT_GELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_GELU, true>), grid, dim3(256), 0, st, p); return;
-            case ACT_SILU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_SILU, true>), grid, dim3(256), 0, st, p); return;
-            default: break;
-        }
+template <typename K> int raise_lds(K kern, size_t lds, std::atomic<bool>* set) {
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    dev &= 63;
+    if (!set[dev].load(std::memory_order_acquire)) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        DIG_CHECK(e == hipSuccess, DIG_ELAUNCH, "linear_act: cannot raise dynamic LDS to %zu: %s", lds, hipGetErrorString(e));
+        set[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL((linear_join_kernel<T, ACT_NONE, FULL>), grid, dim3(256), 0, st, p);
+    return DIG_OK;
+}
+template <int BR, int BC, int NW, int WC, int NS> constexpr size_t lds_of() {
+    constexpr size_t stages = (size_t)NS * (BR + BC) * KB, rows = (size_t)NW * 2 * 16 * (BC / WC + 4) * 4;
+    return stages > rows ? stages : rows;
 }
 
-template <typename T, bool TP, bool TQ, int BR, int BC, int WR, int WC, int NS, bool ALIGNED> int tile_launch(const LinP& p, hipStream_t st) {
-    constexpr bool FULL = !TQ;  // the forward
-    constexpr size_t stages = (size_t)(ALIGNED ? NS : 1) * (BR + BC) * KB, rows = (size_t)WR * WC * 16 * (BC / WC + 4) * 4, lds = stages > rows ? stages : rows;
-    auto kern = linear_kernel<T, TP, TQ, BR, BC, WR, WC, NS, ALIGNED, FULL>;
+// ---- forward
+template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW, bool ALIGNED> int fwd_launch(const LinP& p, hipStream_t st) {
+    constexpr size_t lds = lds_of<BR, BC, WR * WC, WC, ALIGNED ? NS : 1>();
+    auto kern = linear_kernel<T, BR, BC, WR, WC, NS, MINW, ALIGNED>;
     if constexpr (lds > 64 * 1024) {
-        static std::atomic<bool> attr_set[64];
-        int dev = 0;
-        (void)hipGetDevice(&dev);
-        dev &= 63;
-        if (!attr_set[dev].load(std::memory_order_acquire)) {
-            const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            DIG_CHECK(e == hipSuccess, DIG_ELAUNCH, "linear_act: cannot raise dynamic LDS to %zu: %s", lds, hipGetErrorString(e));
-            attr_set[dev].store(true, std::memory_order_release);
+        static std::atomic<bool> set[64];
+        const int rc = raise_lds(kern, lds, set);
+        if (rc != DIG_OK) return rc;
+    }
+    const int rt = up(p.R, BR), ct = up(p.C, BC);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(rt * ct * p.splits)), dim3(WR * WC * 64), lds, st, p, rt, ct);
+    if (p.splits > 1) {
+        const dim3 grid((unsigned)(((long long)p.R * up(p.C, 8) + 255) / 256));
+        switch (p.act) {
+            case ACT_RELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_RELU>), grid, dim3(256), 0, st, p); break;
+            case ACT_GELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_GELU>), grid, dim3(256), 0, st, p); break;
+            case ACT_SILU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_SILU>), grid, dim3(256), 0, st, p); break;
+            default: hipLaunchKernelGGL((linear_join_kernel<T, ACT_NONE>), grid, dim3(256), 0, st, p); break;
         }
     }
-    const int rt = (p.R + BR - 1) / BR, ct = (p.C + BC - 1) / BC;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(rt * ct * p.splits)), dim3(WR * WC * 64), lds, st, p, rt, ct);
-    if (p.splits > 1) join_launch<T, FULL>(p, st);
     DIG_LAUNCH_CHECK("linear_act");
     return DIG_OK;
 }
 
-template <typename T, bool TP, bool TQ> int product(LinP p, bool aligned, hipStream_t st) {
-    constexpr int BK = KB / (int)sizeof(T);
-    split_of(p.R, p.C, p.K, BK, p.splits, p.kper);
-#ifdef NOSPLIT
-    p.splits = 1; p.kper = (p.K + BK - 1) / BK * BK;
+#ifndef FORCE_TILE
+#define FORCE_TILE 0
 #endif
-    // byte offsets inside a tile are 31 bits: 256 rows of k-adjacent operands, BK rows of the others
-    const long long po = (long long)(TP ? BK : 256) * p.ldp, qo = (long long)(TQ ? BK : 256) * p.ldq;
-    if (po * (long long)sizeof(T) >= (1ll << 31) || qo * (long long)sizeof(T) >= (1ll << 31)) aligned = false;
-    if (!aligned) return tile_launch<T, TP, TQ, 128, 128, 2, 2, 2, false>(p, st);
-    if (BIG_TILE) return tile_launch<T, TP, TQ, BT_R, BT_C, BT_WR, BT_WC, (TQ ? 2 : BT_NS), true>(p, st);
-    return tile_launch<T, TP, TQ, 128, 128, 2, 2, 2, true>(p, st);
+enum { TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4 };
+// tile and k slices of the forward
+int fwd_plan(int M, int N, int K, int dtype, int& splits) {
+    splits = 1;
+    if (FORCE_TILE) return FORCE_TILE;
+    return TILE_128;
 }
 
-long long part_floats(int R, int C, int K, int dtype) {
-    int s, kper;
-    split_of(R, C, K, KB / (dtype == DIG_BF16 ? 2 : 4), s, kper);
-    return s > 1 ? (long long)s * R * C : 0;
-}
-
-// rows of a block of the dz kernel: 128 blocks of rows, each thread at most 256 fp32 additions deep until the grid's limit
-int dz_rows(int M) {
-    int rows = (M + 127) / 128;
-    if (rows < 32) rows = 32;
-    if (rows > 1024) rows = 1024;
-    if ((long long)rows * 65535 < M) rows = (int)(((long long)M + 65534) / 65535);
-    return rows;
-}
-int dz_chunks(int M) { return (M + dz_rows(M) - 1) / dz_rows(M); }
-
-bool shape_ok(int M, int N, int K) {
-    return M > 0 && N > 0 && K > 0 && N <= (1 << 20) && K <= (1 << 20) && (long long)((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE) < (1 << 22) &&
-           (long long)((M + TILE - 1) / TILE) * ((K + TILE - 1) / TILE) < (1 << 22);
-}
+// byte offsets inside a tile are 31 bits: up to 256 rows of a k-adjacent operand, the tile's k rows of the others
+bool offsets_ok(long long ld, bool k_adjacent, int esize) { return ld * (k_adjacent ? 256 : KB / esize) * esize < (1ll << 31); }
 
 template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     const int E = 16 / (int)sizeof(T);
@@ -654,8 +683,59 @@ template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     p.pre = a->pre;
     p.act = a->act;
     p.vec = a->N % 8 == 0 && al16(a->out) && (!a->pre || al16(a->pre)) && (!a->res || (al16(a->res) && a->ldr % 8 == 0));
-    const bool aligned = a->K % E == 0 && a->ldx % E == 0 && a->ldw % E == 0 && al16(a->x) && al16(a->w);
-    return product<T, false, false>(p, aligned, st);
+    const bool aligned = a->K % E == 0 && a->ldx % E == 0 && a->ldw % E == 0 && al16(a->x) && al16(a->w) && offsets_ok(a->ldx, true, (int)sizeof(T)) &&
+                         offsets_ok(a->ldw, true, (int)sizeof(T));
+    int splits;
+    const int tile = fwd_plan(a->M, a->N, a->K, a->dtype, splits);
+    set_split(p, splits, KB / (int)sizeof(T));
+    if (!aligned) return fwd_launch<T, 128, 128, 2, 2, 2, 2, false>(p, st);
+    switch (tile) {
+        case TILE_64: return fwd_launch<T, 64, 64, 2, 2, 4, 2, true>(p, st);
+        case TILE_192: return fwd_launch<T, 192, 128, 2, 2, 2, 2, true>(p, st);
+        case TILE_256: return fwd_launch<T, 256, 256, 2, 4, 2, 2, true>(p, st);
+        default: return fwd_launch<T, 128, 128, 2, 2, 2, 2, true>(p, st);
+    }
+}
+
+// ---- backward
+// k slices of dx (nkx k tiles) and dW (nkw): least estimated time of one launch over 512 block slots, in k steps of a block.  A block costs its k tiles
+// and OVER more (fill and epilogue); what is split is written and read again as fp32.
+void bwd_plan(int M, int N, int K, int dtype, bool dx, int& sx, int& sw) {
+    const int bk = KB / (dtype == DIG_BF16 ? 2 : 4), nkx = up(N, bk), nkw = up(M, bk);
+    const double tx = dx ? (double)up(M, TILE) * up(K, TILE) : 0.0, tw = (double)up(N, TILE) * up(K, TILE), OVER = 4.0;
+    const double join = dtype == DIG_BF16 ? 1.0 / (0.75 * 4.0e6) : 1.0 / (3.5 * 4.0e6);  // k steps per byte written and read: a step takes 0.75 (fp32: 3.5) us, a byte 0.25 ps
+    double best = 1e30;
+    sx = sw = 1;
+    for (int a = 1; a <= 4 && (a == 1 || (dx && nkx >= 4 * a)); a++)
+        for (int b = 1; b <= 64 && (b == 1 || nkw >= 4 * b); b++) {
+            const double bx = up(nkx, a) + OVER, bw = up(nkw, b) + OVER, work = tx * a * bx + tw * b * bw, most = (dx && bx > bw) ? bx : bw;
+            double t = work / 512.0 + 0.5 * most;
+            if (t < most) t = most;
+            if (a > 1) t += join * 4.0 * a * M * K * 2;
+            if (b > 1) t += join * 4.0 * b * N * K * 2;
+            if (t < best - 1e-9) {
+                best = t;
+                sx = a;
+                sw = b;
+            }
+        }
+    sx = up(nkx, up(nkx, sx));
+    sw = up(nkw, up(nkw, sw));
+}
+
+// rows of a block of the dz kernel: 128 blocks of rows, each thread at most 256 fp32 additions deep until the grid's limit
+int dz_rows(int M) {
+    int rows = (M + 127) / 128;
+    if (rows < 32) rows = 32;
+    if (rows > 1024) rows = 1024;
+    if ((long long)rows * 65535 < M) rows = (int)(((long long)M + 65534) / 65535);
+    return rows;
+}
+int dz_chunks(int M) { return (M + dz_rows(M) - 1) / dz_rows(M); }
+
+bool shape_ok(int M, int N, int K) {
+    return M > 0 && N > 0 && K > 0 && N <= (1 << 20) && K <= (1 << 20) && (long long)((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE) < (1 << 22) &&
+           (long long)((M + TILE - 1) / TILE) * ((K + TILE - 1) / TILE) < (1 << 22);
 }
 
 template <typename T, int ACT> void dz_launch(const DzP& d, bool vec, dim3 grid, hipStream_t st) {
@@ -663,76 +743,106 @@ template <typename T, int ACT> void dz_launch(const DzP& d, bool vec, dim3 grid,
     else hipLaunchKernelGGL((linear_dz_kernel<T, 1, ACT>), grid, dim3(256), 0, st, d);
 }
 
+// floats of partial products of dx and dW
+long long bwd_part(int M, int N, int K, int dtype, long long& dx_floats) {
+    int sx, sw;
+    bwd_plan(M, N, K, dtype, true, sx, sw);
+    dx_floats = sx > 1 ? (long long)sx * M * K : 0;
+    long long most = dx_floats + (sw > 1 ? (long long)sw * N * K : 0);
+    bwd_plan(M, N, K, dtype, false, sx, sw);  // the same workspace serves a call without dx
+    const long long alone = sw > 1 ? (long long)sw * N * K : 0;
+    if (alone > most) most = alone;
+    dx_floats = (dx_floats + 3) / 4 * 4;
+    return (most + 7) / 4 * 4;
+}
+
 template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) {
-    const int E = 16 / (int)sizeof(T), M = a->M, N = a->N, K = a->K, ldz = (N + 7) / 8 * 8;
+    const int E = 16 / (int)sizeof(T), es = (int)sizeof(T), M = a->M, N = a->N, K = a->K, ldz = up(N, 8) * 8;
     const int chunks = dz_chunks(M);
-    float* part = a->ws;                                    // partial products
-    float* sums = a->ws + dig_linear_act_bwd_part(M, N, K, a->dtype);  // column sums of row blocks
-    if (a->dz || a->db) {
-        DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, a->db ? sums : nullptr, M, N, ldz, dz_rows(M)};
-        const bool vec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre))) && (!a->dz || al16(a->dz));
-        const int width = a->dz ? ldz : N;
-        const dim3 grid((unsigned)(vec ? (width + 511) / 512 : (width + 63) / 64), (unsigned)chunks);
+    long long xf;
+    const long long pf = bwd_part(M, N, K, a->dtype, xf);
+    float* sums = a->ws + pf;  // column sums of row blocks
+    const DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, a->db ? sums : nullptr, M, N, ldz, dz_rows(M)};
+    const bool dvec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre))) && (!a->dz || al16(a->dz));
+    const int width = a->dz ? ldz : N, dcols = dvec ? up(width, 512) : up(width, 64);
+    if (a->dz) {
+        const dim3 grid((unsigned)dcols, (unsigned)chunks);
         switch (a->act) {
-            case ACT_RELU: dz_launch<T, ACT_RELU>(d, vec, grid, st); break;
-            case ACT_GELU: dz_launch<T, ACT_GELU>(d, vec, grid, st); break;
-            case ACT_SILU: dz_launch<T, ACT_SILU>(d, vec, grid, st); break;
-            default: dz_launch<T, ACT_NONE>(d, vec, grid, st); break;
+            case ACT_RELU: dz_launch<T, ACT_RELU>(d, dvec, grid, st); break;
+            case ACT_GELU: dz_launch<T, ACT_GELU>(d, dvec, grid, st); break;
+            case ACT_SILU: dz_launch<T, ACT_SILU>(d, dvec, grid, st); break;
+            default: dz_launch<T, ACT_NONE>(d, dvec, grid, st); break;
         }
-        if (a->db) hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, sums, a->db, chunks, N);
-        DIG_LAUNCH_CHECK("linear_act_bwd");
     }
     const void* dz = a->dz ? a->dz : a->dy;
     const long long lz = a->dz ? ldz : a->ldy;
-    const bool z_ok = lz % E == 0 && al16(dz) && (a->dz || N % E == 0);
-    const bool x_ok = K % E == 0 && a->ldx % E == 0 && al16(a->x), w_ok = K % E == 0 && a->ldw % E == 0 && al16(a->w);
-    if (a->dx) {  // dx[m][k] = sum_n dz[m][n] W[n][k]
-        LinP p{};
-        p.p = dz;
-        p.ldp = lz;
-        p.q = a->w;
-        p.ldq = a->ldw;
-        p.R = M;
-        p.C = p.cpad = K;
-        p.K = N;
-        p.out = a->dx;
-        p.ldo = K;
-        p.part = part;
-        p.vec = K % 8 == 0 && al16(a->dx);
-        const int rc = product<T, false, true>(p, z_ok && w_ok, st);
-        if (rc != DIG_OK) return rc;
+    const bool aligned = lz % E == 0 && al16(dz) && (a->dz || N % E == 0) && K % E == 0 && a->ldx % E == 0 && al16(a->x) && offsets_ok(lz, true, es) && offsets_ok(a->ldx, false, es) &&
+                         (!a->dx || (a->ldw % E == 0 && al16(a->w) && offsets_ok(a->ldw, false, es)));
+    BwdP p{};
+    int sx, sw;
+    bwd_plan(M, N, K, a->dtype, a->dx != nullptr, sx, sw);
+    p.w.p = p.x.p = dz;  // dW[n][k] = sum_m dz[m][n] x[m][k],  dx[m][k] = sum_n dz[m][n] W[n][k]
+    p.w.ldp = p.x.ldp = lz;
+    p.w.q = a->x;
+    p.w.ldq = a->ldx;
+    p.x.q = a->w;
+    p.x.ldq = a->ldw;
+    p.w.R = N;
+    p.w.rpad = a->dz ? ldz : N;
+    p.x.R = M;
+    p.w.C = p.w.cpad = p.x.C = p.x.cpad = K;
+    p.w.K = M;
+    p.x.K = N;
+    p.w.out = a->dw;
+    p.x.out = a->dx;
+    p.w.ldo = p.x.ldo = K;
+    p.w.out_f32 = a->dw_f32;
+    p.w.vec = K % 8 == 0 && al16(a->dw);
+    p.x.vec = K % 8 == 0 && al16(a->dx);
+    p.x.part = a->ws;
+    p.w.part = a->ws + (a->dx ? xf : 0);
+    set_split(p.w, sw, KB / es);
+    set_split(p.x, sx, KB / es);
+    p.wr = up(N, TILE);
+    p.wc = p.xc = up(K, TILE);
+    p.xr = a->dx ? up(M, TILE) : 0;
+    p.w_first = !a->dx || p.w.kper >= p.x.kper;
+    const int nw = up(p.wr * p.wc * p.w.splits, 8) * 8, nx = up(p.xr * p.xc * p.x.splits, 8) * 8;
+    p.n0 = p.w_first ? nw : nx;
+    p.n1 = nw + nx;
+    const bool sum_here = a->db && !a->dz;
+    p.s = d;
+    p.sx = dcols;
+    const dim3 grid((unsigned)(p.n1 + (sum_here ? dcols * chunks : 0)));
+    constexpr size_t lds = lds_of<TILE, TILE, 4, 2, 2>();
+    static_assert(lds <= 64 * 1024, "no attribute needed");
+    if (aligned) {
+        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, true, 8>), grid, dim3(256), lds, st, p);
+        else hipLaunchKernelGGL((linear_bwd_kernel<T, true, 1>), grid, dim3(256), lds, st, p);
+    } else {
+        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, false, 8>), grid, dim3(256), lds, st, p);
+        else hipLaunchKernelGGL((linear_bwd_kernel<T, false, 1>), grid, dim3(256), lds, st, p);
     }
-    LinP p{};  // dW[n][k] = sum_m dz[m][n] x[m][k]
-    p.p = dz;
-    p.ldp = lz;
-    p.q = a->x;
-    p.ldq = a->ldx;
-    p.R = N;
-    p.rpad = a->dz ? ldz : N;
-    p.C = p.cpad = K;
-    p.K = M;
-    p.out = a->dw;
-    p.ldo = K;
-    p.part = part;
-    p.out_f32 = a->dw_f32;
-    p.vec = K % 8 == 0 && al16(a->dw);
-    return product<T, true, true>(p, z_ok && x_ok, st);
+    auto join_blocks = [](const LinP& q) { return q.splits > 1 ? (int)(((long long)q.R * up(q.C, 8) + 255) / 256) : 0; };
+    const int jw = join_blocks(p.w), jx = a->dx ? join_blocks(p.x) : 0, jd = a->db ? up(N, 16) : 0;
+    if (jw + jx + jd) hipLaunchKernelGGL((linear_bwd_join_kernel<T>), dim3((unsigned)(jw + jx + jd)), dim3(256), 0, st, p.w, p.x, jw, jx, sums, a->db, chunks, N);
+    DIG_LAUNCH_CHECK("linear_act_bwd");
+    return DIG_OK;
 }
 
 }  // namespace
 
 extern "C" int dig_linear_act_ws(int M, int N, int K, int dtype) {
     if (!shape_ok(M, N, K)) return DIG_EINVAL;
-    return (int)part_floats(M, N, K, dtype);
-}
-extern "C" int dig_linear_act_bwd_part(int M, int N, int K, int dtype) {
-    if (!shape_ok(M, N, K) || !shape_ok(N, K, 1)) return DIG_EINVAL;
-    const long long a = part_floats(M, K, N, dtype), b = part_floats(N, K, M, dtype);
-    return (int)(((a > b ? a : b) + 3) / 4 * 4);
+    int s;
+    (void)fwd_plan(M, N, K, dtype, s);
+    return s > 1 ? (int)((long long)s * M * N) : 0;
 }
 extern "C" int dig_linear_act_bwd_ws(int M, int N, int K, int dtype) {
-    const int part = dig_linear_act_bwd_part(M, N, K, dtype);
-    return part < 0 ? part : part + dz_chunks(M) * N;
+    if (!shape_ok(M, N, K) || !shape_ok(N, K, 1)) return DIG_EINVAL;
+    long long xf;
+    const long long n = bwd_part(M, N, K, dtype, xf) + (long long)dz_chunks(M) * N;
+    return n < (1ll << 31) ? (int)n : DIG_EINVAL;
 }
 
 extern "C" int dig_linear_act(const dig_linear_act_args* a, void* stream) {

@@ -873,8 +873,8 @@ int dig_linear_act_ws(int M, int N, int K, int dtype);
 
 /* adjoint: dz = dy * act'(pre),  dx = dz w (NULL: not wanted),  dw = dz^T x (dtype, or fp32 if dw_f32),  db = column sums of dz, fp32
  * (NULL: no bias); all outputs contiguous.  dz: [M][N rounded up to 8] of dtype, workspace; may be NULL when act is DIG_ACT_NONE (dy is then
- * multiplied as it lies; with dz given it is copied there first, which aligns it).  ws: dig_linear_act_bwd_ws(...) floats, of which
- * the first dig_linear_act_bwd_part(...) hold partial products.  The residual's gradient is dy itself. */
+ * multiplied as it lies; with dz given it is copied there first, which aligns it).  ws: dig_linear_act_bwd_ws(...) floats.
+ * The residual's gradient is dy itself. */
 typedef struct {
     const void* x;
     const void* w;
@@ -889,7 +889,6 @@ typedef struct {
     int M, N, K, act, dtype, dw_f32;
 } dig_linear_act_bwd_args;
 int dig_linear_act_bwd(const dig_linear_act_bwd_args* a, void* stream);
-int dig_linear_act_bwd_part(int M, int N, int K, int dtype);
 int dig_linear_act_bwd_ws(int M, int N, int K, int dtype);
 
 #ifdef __cplusplus
