@@ -43,52 +43,46 @@ template <bool FULL> __device__ __forceinline__ void load_bias(const LinP& p, in
     for (int j = 0; j < 8; j++) bias[j] = FULL && p.bias && c + j < p.C ? p.bias[c + j] : 0.f;
 }
 
-// 8 columns of the epilogue from column c of row r: n of them exist.  FULL: bias, pre, act and res; otherwise only the store.  rv: the
-// residual's vector, if p.vec
-template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(const LinP& p, float (&v)[8], int r, int c, int n, const Frag<T>& rv, const float (&bias)[8]) {
+// 8 columns of the epilogue from column c of row r (p.vec).  FULL: bias, pre, act and res; otherwise only the store.  rv: the residual's vector
+template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi8(const LinP& p, float (&v)[8], int r, int c, const Frag<T>& rv, const float (&bias)[8]) {
     const size_t o = (size_t)r * p.ldo + c;
-    if (p.vec) {  // n is 8
-        Frag<T> f;
-        if constexpr (FULL) {
+    Frag<T> f;
+    if constexpr (FULL) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] += bias[j];
-            if (p.pre) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) frag_set<T>(f, j, v[j]);
-                frag_store<T>(f, (T*)p.pre + o);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = act_val<T, ACT>(v[j]);
-            if (p.res) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] += frag_get<T>(rv, j);
-            }
-        }
-        if (p.out_f32) {
-            float* d = (float*)p.out + o;
-            *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
+        for (int j = 0; j < 8; j++) v[j] += bias[j];
+        if (p.pre) {
 #pragma unroll
             for (int j = 0; j < 8; j++) frag_set<T>(f, j, v[j]);
-            frag_store<T>(f, (T*)p.out + o);
+            frag_store<T>(f, (T*)p.pre + o);
         }
-        return;
-    }
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        if (j < n) {
-            float z = v[j];
-            if constexpr (FULL) {
-                z += bias[j];
-                if (p.pre) ((T*)p.pre)[o + j] = from_f32<T>(z);
-                z = act_val<T, ACT>(z);
-                if (p.res) z += to_f32<T>(((const T*)p.res)[(size_t)r * p.ldr + c + j]);
-            }
-            if (p.out_f32) ((float*)p.out)[o + j] = z;
-            else ((T*)p.out)[o + j] = from_f32<T>(z);
+        for (int j = 0; j < 8; j++) v[j] = act_val<T, ACT>(v[j]);
+        if (p.res) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] += frag_get<T>(rv, j);
         }
     }
+    if (p.out_f32) {
+        float* d = (float*)p.out + o;
+        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) frag_set<T>(f, j, v[j]);
+        frag_store<T>(f, (T*)p.out + o);
+    }
+}
+// one value, where rows do not start on 16 bytes
+template <typename T, int ACT, bool FULL> __device__ __forceinline__ void epi1(const LinP& p, float z, int r, int c) {
+    const size_t o = (size_t)r * p.ldo + c;
+    if constexpr (FULL) {
+        if (p.bias) z += p.bias[c];
+        if (p.pre) ((T*)p.pre)[o] = from_f32<T>(z);
+        z = act_val<T, ACT>(z);
+        if (p.res) z += to_f32<T>(((const T*)p.res)[(size_t)r * p.ldr + c]);
+    }
+    if (p.out_f32) ((float*)p.out)[o] = z;
+    else ((T*)p.out)[o] = from_f32<T>(z);
 }
 
 // f(0), ..., f(N - 1) with constant indices: hipcc gives up on unrolling a large body, and an array of accumulators indexed by a variable goes to memory
@@ -173,8 +167,8 @@ template <typename T, bool TR, int X> __device__ __forceinline__ typename Ops<T>
 
 template <int N> __device__ __forceinline__ void dma_wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// Tile BR x BC, WR x WC waves.  ALIGNED: both operands have 16-byte aligned rows whose k (or own index) count is a multiple of 16 bytes;
-// otherwise values are fetched one by one through registers.  FULL: the forward's epilogue.
+// Tile BR x BC, WR x WC waves.  Both operands have 16-byte aligned rows whose k (or own index) count fills them (the host packs others first).
+// FULL: the forward's epilogue.
 //
 // A wave holds the fragments of two K steps: those of the next step are read between the matrix instructions of this one (the order is
 // pinned with sched_barrier: left alone, hipcc sinks the reads to their first use).  One barrier per tile of 128 bytes of k, before its
@@ -182,7 +176,7 @@ template <int N> __device__ __forceinline__ void dma_wait_barrier() { asm volati
 // Both operands k-adjacent: NS tiles in LDS, filled by LDS-DMA; the place of a tile is filled again during its last K step.
 // Otherwise (TQ): two tiles in LDS, filled through registers, which fetch a tile ahead - hipcc waits for every DMA in flight before a transposing
 // read, so the two do not go together.
-template <typename T, bool TP, bool TQ, int BR, int BC, int WR, int WC, int NS, bool ALIGNED, bool FULL>
+template <typename T, bool TP, bool TQ, int BR, int BC, int WR, int WC, int NS, bool FULL>
 __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctiles, int id, unsigned char* smem) {
     using SP = Side<T, TP, BR>;
     using SQ = Side<T, TQ, BC>;
@@ -225,7 +219,7 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
     auto pfrag = [&](const unsigned char* st, int i, int kk) { return frag_at<T, TP, BR>(st, wr * (BR / WR) + i * 16, kk, lane); };
     auto qfrag = [&](const unsigned char* st, int j, int kk) { return frag_at<T, TQ, BC>(st + SP::BYTES, wc * WCOLS + j * 16, kk, lane); };
 
-    if constexpr (ALIGNED) {
+    {
         // this lane's pieces: byte offset from the tile's corner at its first k (the host checks that it fits in 31 bits), k within the tile
         unsigned poff[PN], qoff[QN];
         int pk[PN], qk[QN];
@@ -328,49 +322,6 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
             nxt = cur == smem + (NS - 1) * STAGE ? smem : cur + STAGE;
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the last of them have landed before LDS is used again
-    } else {
-        // a piece's values one by one, zero past the end of k (and of the own index, where the next row begins)
-        auto fetch = [&](const T* X, long long ld, int off, int x, int k, bool tr, int lim, int left, unsigned char* st) {
-            T v[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool ok = tr ? k < left && x + e < lim : k + e < left && x < lim;
-                v[e] = ok ? X[tr ? (size_t)k * ld + x + e : (size_t)x * ld + k + e] : from_f32<T>(0.f);
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) reinterpret_cast<T*>(st + off)[e] = v[e];
-        };
-        for (int kt = 0; kt < nk; kt++) {
-            const int left = kend - kbeg - kt * BK;
-#pragma unroll
-            for (int j = 0; j < PN; j++) {
-                const int off = (wave + j * NW) * 1024 + lane * 16;
-                int x, k;
-                SP::piece(off, x, k);
-                fetch(P + (TP ? (size_t)kt * BK * p.ldp : (size_t)kt * BK), p.ldp, off, x, k, TP, p.R - r0, left, smem);
-            }
-#pragma unroll
-            for (int j = 0; j < QN; j++) {
-                const int off = (wave + j * NW) * 1024 + lane * 16;
-                int x, k;
-                SQ::piece(off, x, k);
-                fetch(Q + (TQ ? (size_t)kt * BK * p.ldq : (size_t)kt * BK), p.ldq, off, x, k, TQ, p.C - c0, left, smem + SP::BYTES);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                F fp[TRN], fq[TCN];
-#pragma unroll
-                for (int i = 0; i < TRN; i++) fp[i] = pfrag(smem, i, kk);
-#pragma unroll
-                for (int j = 0; j < TCN; j++) fq[j] = qfrag(smem, j, kk);
-#pragma unroll
-                for (int i = 0; i < TRN; i++)
-#pragma unroll
-                    for (int j = 0; j < TCN; j++) Ops<T>::mma(acc[i][j], fq[j], fp[i]);
-            }
-            __syncthreads();
-        }
     }
 
     // ---- epilogue: 16 rows of the wave's columns at a time through LDS rows of its own (two sets: the next rows are written while these
@@ -420,23 +371,29 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
                 if (use_res) fetch_res(i + 1);
             }
             __builtin_amdgcn_wave_barrier();
+            if (p.vec) {
 #pragma unroll
-            for (int it = 0; it < ITEMS; it++) {
-                const int r = rfirst + i * 16 + it * STEP;
-                if (r < p.R && n > 0) {
-                    float v[8] = {a[it][0], a[it][1], a[it][2], a[it][3], b[it][0], b[it][1], b[it][2], b[it][3]};
-                    if (part) {
-                        float* d = part + (size_t)r * p.C + c;
-                        if (n == 8 && p.C % 4 == 0) {
+                for (int it = 0; it < ITEMS; it++) {
+                    const int r = rfirst + i * 16 + it * STEP;
+                    if (r < p.R && n > 0) {
+                        float v[8] = {a[it][0], a[it][1], a[it][2], a[it][3], b[it][0], b[it][1], b[it][2], b[it][3]};
+                        if (part) {
+                            float* d = part + (size_t)r * p.C + c;
                             *reinterpret_cast<f32x4*>(d) = a[it];
                             *reinterpret_cast<f32x4*>(d + 4) = b[it];
                         } else {
-#pragma unroll
-                            for (int e = 0; e < 8; e++)
-                                if (e < n) d[e] = v[e];
+                            epi8<T, ACT, FULL>(p, v, r, c, rv[it], bias);
                         }
-                    } else {
-                        epi8<T, ACT, FULL>(p, v, r, c, n, rv[it], bias);
+                    }
+                }
+            } else {  // value by value, adjacent lanes on adjacent columns
+#pragma unroll
+                for (int it = 0; it < 16 * WCOLS / 64; it++) {
+                    const int e = it * 64 + lane, y = e / WCOLS, x = e % WCOLS, r = r0 + wr * (BR / WR) + i * 16 + y, cc = c0 + wc * WCOLS + x;
+                    const float z = ot[(i & 1) * 16 * OS + y * OS + x];
+                    if (r < p.R && cc < p.C) {
+                        if (part) part[(size_t)r * p.C + cc] = z;
+                        else epi1<T, ACT, FULL>(p, z, r, cc);
                     }
                 }
             }
@@ -454,9 +411,122 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
 
 // MINW waves per SIMD: it bounds the registers, and with at most 256 of them hipcc keeps the accumulators where the matrix instructions read them (with
 // more it moves them between the two register files in every K step)
-template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW, bool ALIGNED> __global__ __launch_bounds__(WR* WC * 64, MINW) void linear_kernel(LinP p, int rtiles, int ctiles) {
+template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> __global__ __launch_bounds__(WR* WC * 64, MINW) void linear_kernel(LinP p, int rtiles, int ctiles) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    linear_tile<T, false, false, BR, BC, WR, WC, NS, ALIGNED, true>(p, rtiles, ctiles, blockIdx.x, smem);
+    linear_tile<T, false, false, BR, BC, WR, WC, NS, true>(p, rtiles, ctiles, blockIdx.x, smem);
+}
+
+// ---- few outputs: a block takes 32 x 32 of them, its four waves every fourth K step.  The fragments come straight from memory (the operands are
+// small and shared through L2), all of a wave's loads for 4 steps in flight; the partial sums meet in LDS.  No k slices over blocks, so
+// one launch: 20x384x1536 fp32 takes ... ALIGNED as above; otherwise value by value.
+template <typename T, bool ALIGNED> __global__ __launch_bounds__(256) void linear_small_kernel(LinP p, int ctiles) {
+    using F = typename Ops<T>::F;
+    constexpr int E = 16 / (int)sizeof(T), KK = Ops<T>::KK, OS = 36;
+    __shared__ float sm[4][32 * OS];
+    const int rt = blockIdx.x / ctiles, r0 = rt * 32, c0 = (blockIdx.x - rt * ctiles) * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q4 = lane >> 4;
+    const T *ps[2], *qs[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        ps[i] = (const T*)p.p + (size_t)min(r0 + i * 16 + i16, p.R - 1) * p.ldp + q4 * E;
+        qs[i] = (const T*)p.q + (size_t)min(c0 + i * 16 + i16, p.C - 1) * p.ldq + q4 * E;
+    }
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const T* src, int k) {  // E values from k + q4 E on; zero past the end
+        F f = {};
+        const int left = p.K - (k + q4 * E);
+        if constexpr (ALIGNED) {
+            if (left > 0) f = *reinterpret_cast<const F*>(src + k);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (e < left) f[e] = src[k + e];
+        }
+        return f;
+    };
+    constexpr int U = 4;
+    const int steps = (p.K + KK - 1) / KK;
+    for (int s = wave; s < steps; s += 4 * U) {
+        F fp[U][2], fq[U][2];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {  // steps past the end load zeros
+                fp[u][i] = load(ps[i], (s + 4 * u) * KK);
+                fq[u][i] = load(qs[i], (s + 4 * u) * KK);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) Ops<T>::mma(acc[i][j], fq[u][j], fp[u][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) *reinterpret_cast<f32x4*>(&sm[wave][(i * 16 + i16) * OS + j * 16 + q4 * 4]) = acc[i][j];
+    __syncthreads();
+    // adjacent lanes on adjacent columns: 8 rows at a time
+#pragma unroll
+    for (int it = 0; it < 4; it++) {
+        const int y = it * 8 + (threadIdx.x >> 5), x = threadIdx.x & 31, r = r0 + y, c = c0 + x, o = y * OS + x;
+        if (r >= p.R || c >= p.C) continue;
+        const float z = (sm[0][o] + sm[1][o]) + (sm[2][o] + sm[3][o]);
+        if (p.act == ACT_RELU) epi1<T, ACT_RELU, true>(p, z, r, c);
+        else if (p.act == ACT_GELU) epi1<T, ACT_GELU, true>(p, z, r, c);
+        else if (p.act == ACT_SILU) epi1<T, ACT_SILU, true>(p, z, r, c);
+        else epi1<T, ACT_NONE, true>(p, z, r, c);
+    }
+}
+
+// ---- operands whose rows do not lie on 16 bytes, copied to rows that do (zeros behind them): a thread moves 16 bytes
+struct PackP {
+    const void* src[2];
+    void* dst[2];
+    long long ld[2];
+    long long n[2];  // 16-byte pieces; 0: nothing to do
+    int K, per_row;  // values and pieces of a row
+};
+template <typename T> __device__ __forceinline__ void pack1(const T* src, T* dst, int left) {
+    constexpr int E = 16 / (int)sizeof(T);
+    unsigned w[4] = {0, 0, 0, 0};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (e < left) w[e] = __builtin_bit_cast(unsigned, src[e]);
+    } else {  // whole words that hold at least one of the values, shifted into place
+        const bool odd = ((uintptr_t)src & 2) != 0;
+        const unsigned* q = reinterpret_cast<const unsigned*>((uintptr_t)src & ~(uintptr_t)3);
+        unsigned v[5];
+        const int have = min(left, E) + (odd ? 1 : 0);  // halves from q on
+#pragma unroll
+        for (int e = 0; e < 5; e++) v[e] = 2 * e < have ? q[e] : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = odd ? (v[e] >> 16) | (v[e + 1] << 16) : v[e];
+            if (2 * e >= left) w[e] = 0;
+            else if (2 * e + 1 >= left) w[e] &= 0xffffu;
+        }
+    }
+    *reinterpret_cast<f32x4*>(dst) = f32x4{__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]), __builtin_bit_cast(float, w[2]), __builtin_bit_cast(float, w[3])};
+}
+template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackP p) {
+    constexpr int E = 16 / (int)sizeof(T);
+    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    int which = 0;
+    if (i >= p.n[0]) {
+        i -= p.n[0];
+        which = 1;
+    }
+    if (i >= p.n[which]) return;
+    const long long r = i / p.per_row;
+    const int k = (int)(i - r * p.per_row) * E;
+    pack1<T>((const T*)p.src[which] + r * p.ld[which] + k, (T*)p.dst[which] + i * E, p.K - k);
 }
 
 // splits > 1: the partial products of a row's 8 columns, added in order, and the epilogue
@@ -468,7 +538,7 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const float* s = p.part + (size_t)r * p.C + c;
     const size_t step = (size_t)p.R * p.C;
-    if (n == 8 && p.C % 4 == 0) {
+    if (p.vec) {  // n is 8
 #pragma unroll 4
         for (int k = 0; k < p.splits; k++) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(s + k * step), b = *reinterpret_cast<const f32x4*>(s + k * step + 4);
@@ -478,17 +548,20 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear
                 v[4 + e] += b[e];
             }
         }
+        Frag<T> rv;
+        if (FULL && p.res) frag_load<T>(rv, (const T*)p.res + (size_t)r * p.ldr + c);
+        float bias[8];
+        load_bias<FULL>(p, c, bias);
+        epi8<T, ACT, FULL>(p, v, r, c, rv, bias);
     } else {
         for (int k = 0; k < p.splits; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 if (e < n) v[e] += s[k * step + e];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) epi1<T, ACT, FULL>(p, v[e], r, c + e);
     }
-    Frag<T> rv;
-    if (FULL && p.res && p.vec) frag_load<T>(rv, (const T*)p.res + (size_t)r * p.ldr + c);
-    float bias[8];
-    load_bias<FULL>(p, c, bias);
-    epi8<T, ACT, FULL>(p, v, r, c, n, rv, bias);
 }
 template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) { linear_join<T, ACT, true>(p, blockIdx.x); }
 
@@ -566,7 +639,7 @@ __device__ __forceinline__ void linear_db(const float* part, float* db, int chun
 }
 
 // ---- the products of the backward in one launch: the blocks of dW, those of dx and, without an activation, those of the column sums of dy.
-// Two 128 x 128 blocks per CU; one launch fills the chip where dW (few tiles, long k) or dx alone would not, and the tails overlap.
+// Tiles of TL x TL, two 128 x 128 blocks per CU; one launch fills the chip where dW (few tiles, long k) or dx alone would not, and the tails overlap.
 struct BwdP {
     LinP w, x;
     int wr, wc, xr, xc;           // tiles
@@ -575,7 +648,7 @@ struct BwdP {
     DzP s;
     int sx;                       // column blocks of the sums
 };
-template <typename T, bool ALIGNED, int SV> __global__ __launch_bounds__(256, 2) void linear_bwd_kernel(BwdP p) {
+template <typename T, int TL, int SV> __global__ __launch_bounds__(256, 2) void linear_bwd_kernel(BwdP p) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int id = blockIdx.x;
     if (id >= p.n1) {
@@ -585,9 +658,9 @@ template <typename T, bool ALIGNED, int SV> __global__ __launch_bounds__(256, 2)
     const bool first = id < p.n0;
     const int at = first ? id : id - p.n0;
     if (first == (p.w_first != 0)) {
-        if (at < p.wr * p.wc * p.w.splits) linear_tile<T, true, true, 128, 128, 2, 2, 2, ALIGNED, false>(p.w, p.wr, p.wc, at, smem);
+        if (at < p.wr * p.wc * p.w.splits) linear_tile<T, true, true, TL, TL, 2, 2, 2, false>(p.w, p.wr, p.wc, at, smem);
     } else {
-        if (at < p.xr * p.xc * p.x.splits) linear_tile<T, false, true, 128, 128, 2, 2, 2, ALIGNED, false>(p.x, p.xr, p.xc, at, smem);
+        if (at < p.xr * p.xc * p.x.splits) linear_tile<T, false, true, TL, TL, 2, 2, 2, false>(p.x, p.xr, p.xc, at, smem);
     }
 }
 // what remains: the joins of dW and dx, and db from the column sums
@@ -627,9 +700,9 @@ template <int BR, int BC, int NW, int WC, int NS> constexpr size_t lds_of() {
 }
 
 // ---- forward
-template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW, bool ALIGNED> int fwd_launch(const LinP& p, hipStream_t st) {
-    constexpr size_t lds = lds_of<BR, BC, WR * WC, WC, ALIGNED ? NS : 1>();
-    auto kern = linear_kernel<T, BR, BC, WR, WC, NS, MINW, ALIGNED>;
+template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> int fwd_launch(const LinP& p, hipStream_t st) {
+    constexpr size_t lds = lds_of<BR, BC, WR * WC, WC, NS>();
+    auto kern = linear_kernel<T, BR, BC, WR, WC, NS, MINW>;
     if constexpr (lds > 64 * 1024) {
         static std::atomic<bool> set[64];
         const int rc = raise_lds(kern, lds, set);
@@ -651,26 +724,80 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW, bool ALI
 }
 
 #ifndef FORCE_TILE
-#define FORCE_TILE 0
+#define FORCE_TILE -1
 #endif
-enum { TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4 };
-// tile and k slices of the forward
+enum { TILE_SMALL = 0, TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4 };
+// Tile and k slices of the forward: the least estimated time.  A block of a tile costs fill + k tiles * step us while its CU holds as many
+// blocks as fit (slots in all); measured at 5864x384x81, 6912x384x1536 and 8192x4096x4096 in bf16 (64: 7.2 / 35 / 527 us, 128: 12.8 / 27 / 324, 192x128: 17 /
+// 24.5 / 311, 256: 23 / 29 / 245); fp32 steps are the matrix units' own time.  Few outputs take linear_small_kernel; few outputs of a long
+// sum are cut into k slices of 64 x 64 tiles, whose join costs a launch and the partial sums' bytes.
 int fwd_plan(int M, int N, int K, int dtype, int& splits) {
+    struct Cost {
+        int br, bc, slots;
+        double fill, step, step_f32;
+    };
+    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 15.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 7.0}};
+    const bool f32 = dtype != DIG_BF16;
+    const int nk = up(K, f32 ? 32 : 64);
     splits = 1;
-    if (FORCE_TILE) return FORCE_TILE;
-    return TILE_128;
+    if (FORCE_TILE >= 0) return FORCE_TILE;
+    const long long small = (long long)up(M, 32) * up(N, 32);
+    double best = small <= 512 ? (3.0 + up(K, f32 ? 256 : 512) * (f32 ? 1.5 : 1.2)) * (small <= 256 ? 1.0 : 1.6) : 1e30;
+    int tile = TILE_SMALL;
+    for (int i = 0; i < 4; i++) {
+        const double tiles = (double)up(M, cost[i].br) * up(N, cost[i].bc), full = tiles / cost[i].slots;
+        double rounds = full <= 1.0 ? 1.0 : full + 0.4;
+        if (full > 1.0 && rounds > (double)(long long)full + 1.0) rounds = (double)(long long)full + 1.0;
+        const double t = rounds * (cost[i].fill + nk * (f32 ? cost[i].step_f32 : cost[i].step));
+        if (t < best) {
+            best = t;
+            tile = TILE_64 + i;
+        }
+    }
+    const long long t64 = (long long)up(M, 64) * up(N, 64);
+    if (t64 < 256 && nk >= 16) {
+        int n = (int)(512 / t64);
+        if (n > nk / 8) n = nk / 8;
+        if (n > 64) n = 64;
+        n = up(nk, up(nk, n));
+        if (n > 1 && 4.5 + up(nk, n) * (f32 ? 0.9 : 0.445) + 6.0 + 8.0 * n * M * N / 4.5e6 < best) {
+            splits = n;
+            tile = TILE_64;
+        }
+    }
+    return tile;
 }
 
 // byte offsets inside a tile are 31 bits: up to 256 rows of a k-adjacent operand, the tile's k rows of the others
 bool offsets_ok(long long ld, bool k_adjacent, int esize) { return ld * (k_adjacent ? 256 : KB / esize) * esize < (1ll << 31); }
 
+// an operand of 16-byte rows, or its packed copy's place; false: it has to be packed and there is no place for it
+struct Operand {
+    const void* p;
+    long long ld;
+};
+template <typename T> bool operand(const void* src, long long ld, bool k_adjacent, int rows, int K, void* pack, PackP& pp, int slot, Operand& o) {
+    const int E = 16 / (int)sizeof(T);
+    o = {src, ld};
+    if (K % E == 0 && ld % E == 0 && al16(src) && offsets_ok(ld, k_adjacent, (int)sizeof(T))) return true;
+    if (!pack || !al16(pack)) return false;
+    pp.src[slot] = src;
+    pp.dst[slot] = pack;
+    pp.ld[slot] = ld;
+    pp.K = K;
+    pp.per_row = up(K, E);
+    pp.n[slot] = (long long)rows * pp.per_row;
+    o = {pack, (long long)pp.per_row * E};
+    return true;
+}
+template <typename T> void pack_launch(const PackP& pp, hipStream_t st) {
+    const long long n = pp.n[0] + pp.n[1];
+    if (n) hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, pp);
+}
+
 template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     const int E = 16 / (int)sizeof(T);
     LinP p{};
-    p.p = a->x;
-    p.q = a->w;
-    p.ldp = a->ldx;
-    p.ldq = a->ldw;
     p.R = a->M;
     p.C = a->N;
     p.K = a->K;
@@ -683,44 +810,103 @@ template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     p.pre = a->pre;
     p.act = a->act;
     p.vec = a->N % 8 == 0 && al16(a->out) && (!a->pre || al16(a->pre)) && (!a->res || (al16(a->res) && a->ldr % 8 == 0));
-    const bool aligned = a->K % E == 0 && a->ldx % E == 0 && a->ldw % E == 0 && al16(a->x) && al16(a->w) && offsets_ok(a->ldx, true, (int)sizeof(T)) &&
-                         offsets_ok(a->ldw, true, (int)sizeof(T));
     int splits;
     const int tile = fwd_plan(a->M, a->N, a->K, a->dtype, splits);
+    if (tile == TILE_SMALL) {
+        p.p = a->x;
+        p.q = a->w;
+        p.ldp = a->ldx;
+        p.ldq = a->ldw;
+        const int ct = up(p.C, 32);
+        const dim3 grid((unsigned)(up(p.R, 32) * ct));
+        if (a->K % E == 0 && a->ldx % E == 0 && a->ldw % E == 0 && al16(a->x) && al16(a->w)) hipLaunchKernelGGL((linear_small_kernel<T, true>), grid, dim3(256), 0, st, p, ct);
+        else hipLaunchKernelGGL((linear_small_kernel<T, false>), grid, dim3(256), 0, st, p, ct);
+        DIG_LAUNCH_CHECK("linear_act");
+        return DIG_OK;
+    }
+    PackP pp{};
+    Operand x, w;
+    DIG_CHECK(operand<T>(a->x, a->ldx, true, a->M, a->K, a->xpack, pp, 0, x) && operand<T>(a->w, a->ldw, true, a->N, a->K, a->wpack, pp, 1, w), DIG_EALIGN,
+              "linear_act: rows that do not lie on 16 bytes need xpack / wpack");
+    pack_launch<T>(pp, st);
+    p.p = x.p;
+    p.q = w.p;
+    p.ldp = x.ld;
+    p.ldq = w.ld;
     set_split(p, splits, KB / (int)sizeof(T));
-    if (!aligned) return fwd_launch<T, 128, 128, 2, 2, 2, 2, false>(p, st);
     switch (tile) {
-        case TILE_64: return fwd_launch<T, 64, 64, 2, 2, 4, 2, true>(p, st);
-        case TILE_192: return fwd_launch<T, 192, 128, 2, 2, 2, 2, true>(p, st);
-        case TILE_256: return fwd_launch<T, 256, 256, 2, 4, 2, 2, true>(p, st);
-        default: return fwd_launch<T, 128, 128, 2, 2, 2, 2, true>(p, st);
+        case TILE_64: return fwd_launch<T, 64, 64, 2, 2, 4, 2>(p, st);
+        case TILE_192: return fwd_launch<T, 192, 128, 2, 2, 2, 2>(p, st);
+        case TILE_256: return fwd_launch<T, 256, 256, 2, 4, 2, 2>(p, st);
+        default: return fwd_launch<T, 128, 128, 2, 2, 2, 2>(p, st);
     }
 }
 
 // ---- backward
-// k slices of dx (nkx k tiles) and dW (nkw): least estimated time of one launch over 512 block slots, in k steps of a block.  A block costs its k tiles
-// and OVER more (fill and epilogue); what is split is written and read again as fp32.
-void bwd_plan(int M, int N, int K, int dtype, bool dx, int& sx, int& sw) {
-    const int bk = KB / (dtype == DIG_BF16 ? 2 : 4), nkx = up(N, bk), nkw = up(M, bk);
-    const double tx = dx ? (double)up(M, TILE) * up(K, TILE) : 0.0, tw = (double)up(N, TILE) * up(K, TILE), OVER = 4.0;
-    const double join = dtype == DIG_BF16 ? 1.0 / (0.75 * 4.0e6) : 1.0 / (3.5 * 4.0e6);  // k steps per byte written and read: a step takes 0.75 (fp32: 3.5) us, a byte 0.25 ps
+struct BwdPlan {
+    int tile, sx, sw;  // tile 64 or 128, k slices of dx and of dW
+};
+// when n1 blocks of length b1 and then n2 of length b2 <= b1 are done, over `slots` that take the next block as they become free
+double makespan(double n1, double b1, double n2, double b2, double slots) {
+    const double q = (double)(long long)(n1 / slots), rem = n1 - q * slots, t0 = q * b1, t1 = rem > 0 ? t0 + b1 : t0;
+    if (n2 <= 0) return t1;
     double best = 1e30;
-    sx = sw = 1;
-    for (int a = 1; a <= 4 && (a == 1 || (dx && nkx >= 4 * a)); a++)
-        for (int b = 1; b <= 64 && (b == 1 || nkw >= 4 * b); b++) {
-            const double bx = up(nkx, a) + OVER, bw = up(nkw, b) + OVER, work = tx * a * bx + tw * b * bw, most = (dx && bx > bw) ? bx : bw;
-            double t = work / 512.0 + 0.5 * most;
-            if (t < most) t = most;
-            if (a > 1) t += join * 4.0 * a * M * K * 2;
-            if (b > 1) t += join * 4.0 * b * N * K * 2;
-            if (t < best - 1e-9) {
-                best = t;
-                sx = a;
-                sw = b;
+    for (int e = 0; e < 2; e++) {
+        const double base = e ? t1 : t0;
+        double j = (double)(long long)(((q * b1 * slots + rem * b1 + n2 * b2) / slots - base) / b2) - 1.0;
+        if (j < 1.0) j = 1.0;
+        for (int s = 0; s < 4; s++, j += 1.0) {
+            const double t = base + j * b2 + 1e-9;
+            if (t < t1) continue;
+            if ((slots - rem) * (double)(long long)((t - t0) / b2) + rem * (double)(long long)((t - t1) / b2) >= n2) {
+                if (t < best) best = t;
+                break;
             }
         }
-    sx = up(nkx, up(nkx, sx));
-    sw = up(nkw, up(nkw, sw));
+    }
+    return best < 1e30 ? best : t1 + (n2 / slots + 1.0) * b2;
+}
+// The least estimated time of one launch of both products.  A block costs fill + its k tiles * step us (measured on dx of 6912x1536x384 and
+// 6272x1024x4096 in bf16: tile 64 28 / 119 us, tile 128 23 / 82 us; fp32 steps are the matrix units' own time); what is split is written and read again as fp32.
+BwdPlan bwd_search(int M, int N, int K, int dtype, bool dx) {
+    static const int cuts[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64};
+    const bool f32 = dtype != DIG_BF16;
+    const int bk = f32 ? 32 : 64, nkx = up(N, bk), nkw = up(M, bk);
+    BwdPlan plan{128, 1, 1};
+    double best = 1e30;
+    for (int tile = 64; tile <= 128; tile += 64) {
+        const double fill = tile == 64 ? 2.5 : f32 ? 6.0 : 11.0, step = tile == 64 ? (f32 ? 0.95 : 0.58) : (f32 ? 3.6 : 1.1);
+        const double tx = dx ? (double)up(M, tile) * up(K, tile) : 0.0, tw = (double)up(N, tile) * up(K, tile);
+        for (int a = 1; a <= 4; a++) {
+            if (a > 1 && (!dx || nkx < 4 * a || tx * a > 2048)) break;
+            for (int b : cuts) {
+                if (b > 1 && (nkw < 4 * b || tw * b > 2048)) break;
+                const double bx = fill + up(nkx, a) * step, bw = fill + up(nkw, b) * step;
+                double t = !dx || bw >= bx ? makespan(tw * b, bw, tx * a, bx, 512.0) : makespan(tx * a, bx, tw * b, bw, 512.0);
+                if (a > 1) t += 8.0 * a * M * K / 4.5e6;
+                if (b > 1) t += 8.0 * b * N * K / 4.5e6;
+                if (t < best - 1e-9) {
+                    best = t;
+                    plan = {tile, a, b};
+                }
+            }
+        }
+    }
+    plan.sx = up(nkx, up(nkx, plan.sx));
+    plan.sw = up(nkw, up(nkw, plan.sw));
+    return plan;
+}
+// the search takes a few us: a thread remembers its last shapes' plans
+BwdPlan bwd_plan(int M, int N, int K, int dtype, bool dx) {
+    struct Entry {
+        int M, N, K, key;
+        BwdPlan plan;
+    };
+    static thread_local Entry seen[64];
+    const int key = 1 + dtype * 2 + (dx ? 1 : 0);
+    Entry& e = seen[((unsigned)M * 31u + (unsigned)N * 17u + (unsigned)K * 7u + (unsigned)key) & 63];
+    if (e.key != key || e.M != M || e.N != N || e.K != K) e = {M, N, K, key, bwd_search(M, N, K, dtype, dx)};
+    return e.plan;
 }
 
 // rows of a block of the dz kernel: 128 blocks of rows, each thread at most 256 fp32 additions deep until the grid's limit
@@ -743,27 +929,26 @@ template <typename T, int ACT> void dz_launch(const DzP& d, bool vec, dim3 grid,
     else hipLaunchKernelGGL((linear_dz_kernel<T, 1, ACT>), grid, dim3(256), 0, st, d);
 }
 
-// floats of partial products of dx and dW
-long long bwd_part(int M, int N, int K, int dtype, long long& dx_floats) {
-    int sx, sw;
-    bwd_plan(M, N, K, dtype, true, sx, sw);
-    dx_floats = sx > 1 ? (long long)sx * M * K : 0;
-    long long most = dx_floats + (sw > 1 ? (long long)sw * N * K : 0);
-    bwd_plan(M, N, K, dtype, false, sx, sw);  // the same workspace serves a call without dx
-    const long long alone = sw > 1 ? (long long)sw * N * K : 0;
-    if (alone > most) most = alone;
-    dx_floats = (dx_floats + 3) / 4 * 4;
-    return (most + 7) / 4 * 4;
+long long sum_floats(int M, int N) { return up(dz_chunks(M) * N, 4) * 4ll; }
+long long part_floats(const BwdPlan& q, int M, int N, int K, bool dx, long long& dx_floats) {
+    dx_floats = dx && q.sx > 1 ? ((long long)q.sx * M * K + 3) / 4 * 4 : 0;
+    return dx_floats + (q.sw > 1 ? (long long)q.sw * N * K : 0);
 }
 
 template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) {
     const int E = 16 / (int)sizeof(T), es = (int)sizeof(T), M = a->M, N = a->N, K = a->K, ldz = up(N, 8) * 8;
     const int chunks = dz_chunks(M);
-    long long xf;
-    const long long pf = bwd_part(M, N, K, a->dtype, xf);
-    float* sums = a->ws + pf;  // column sums of row blocks
+    float* sums = a->ws;  // column sums of row blocks, then the partial products of dx and dW
+    float* part = a->ws + sum_floats(M, N);
+    PackP pp{};
+    Operand x, w{};
+    DIG_CHECK(operand<T>(a->x, a->ldx, false, M, K, a->xpack, pp, 0, x) && (!a->dx || operand<T>(a->w, a->ldw, false, N, K, a->wpack, pp, 1, w)), DIG_EALIGN,
+              "linear_act_bwd: rows that do not lie on 16 bytes need xpack / wpack");
+    const Operand z = a->dz ? Operand{a->dz, ldz} : Operand{a->dy, a->ldy};
+    DIG_CHECK(z.ld % E == 0 && al16(z.p) && (a->dz || N % E == 0) && offsets_ok(z.ld, true, es), DIG_EALIGN, "linear_act_bwd: rows of dy that do not lie on 16 bytes need dz");
+    pack_launch<T>(pp, st);
     const DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, a->db ? sums : nullptr, M, N, ldz, dz_rows(M)};
-    const bool dvec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre))) && (!a->dz || al16(a->dz));
+    const bool dvec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre)));
     const int width = a->dz ? ldz : N, dcols = dvec ? up(width, 512) : up(width, 64);
     if (a->dz) {
         const dim3 grid((unsigned)dcols, (unsigned)chunks);
@@ -774,23 +959,21 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
             default: dz_launch<T, ACT_NONE>(d, dvec, grid, st); break;
         }
     }
-    const void* dz = a->dz ? a->dz : a->dy;
-    const long long lz = a->dz ? ldz : a->ldy;
-    const bool aligned = lz % E == 0 && al16(dz) && (a->dz || N % E == 0) && K % E == 0 && a->ldx % E == 0 && al16(a->x) && offsets_ok(lz, true, es) && offsets_ok(a->ldx, false, es) &&
-                         (!a->dx || (a->ldw % E == 0 && al16(a->w) && offsets_ok(a->ldw, false, es)));
+    const BwdPlan plan = bwd_plan(M, N, K, a->dtype, a->dx != nullptr);
+    long long xf;
+    (void)part_floats(plan, M, N, K, a->dx != nullptr, xf);
     BwdP p{};
-    int sx, sw;
-    bwd_plan(M, N, K, a->dtype, a->dx != nullptr, sx, sw);
-    p.w.p = p.x.p = dz;  // dW[n][k] = sum_m dz[m][n] x[m][k],  dx[m][k] = sum_n dz[m][n] W[n][k]
-    p.w.ldp = p.x.ldp = lz;
-    p.w.q = a->x;
-    p.w.ldq = a->ldx;
-    p.x.q = a->w;
-    p.x.ldq = a->ldw;
+    p.w.p = p.x.p = z.p;  // dW[n][k] = sum_m dz[m][n] x[m][k],  dx[m][k] = sum_n dz[m][n] W[n][k]
+    p.w.ldp = p.x.ldp = z.ld;
+    p.w.q = x.p;
+    p.w.ldq = x.ld;
+    p.x.q = w.p;
+    p.x.ldq = w.ld;
     p.w.R = N;
-    p.w.rpad = a->dz ? ldz : N;
+    p.w.rpad = up(N, E) * E;
     p.x.R = M;
-    p.w.C = p.w.cpad = p.x.C = p.x.cpad = K;
+    p.w.C = p.x.C = K;
+    p.w.cpad = p.x.cpad = up(K, E) * E;
     p.w.K = M;
     p.x.K = N;
     p.w.out = a->dw;
@@ -799,13 +982,13 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
     p.w.out_f32 = a->dw_f32;
     p.w.vec = K % 8 == 0 && al16(a->dw);
     p.x.vec = K % 8 == 0 && al16(a->dx);
-    p.x.part = a->ws;
-    p.w.part = a->ws + (a->dx ? xf : 0);
-    set_split(p.w, sw, KB / es);
-    set_split(p.x, sx, KB / es);
-    p.wr = up(N, TILE);
-    p.wc = p.xc = up(K, TILE);
-    p.xr = a->dx ? up(M, TILE) : 0;
+    p.x.part = part;
+    p.w.part = part + xf;
+    set_split(p.w, plan.sw, KB / es);
+    set_split(p.x, plan.sx, KB / es);
+    p.wr = up(N, plan.tile);
+    p.wc = p.xc = up(K, plan.tile);
+    p.xr = a->dx ? up(M, plan.tile) : 0;
     p.w_first = !a->dx || p.w.kper >= p.x.kper;
     const int nw = up(p.wr * p.wc * p.w.splits, 8) * 8, nx = up(p.xr * p.xc * p.x.splits, 8) * 8;
     p.n0 = p.w_first ? nw : nx;
@@ -814,14 +997,14 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
     p.s = d;
     p.sx = dcols;
     const dim3 grid((unsigned)(p.n1 + (sum_here ? dcols * chunks : 0)));
-    constexpr size_t lds = lds_of<TILE, TILE, 4, 2, 2>();
+    constexpr size_t lds = lds_of<128, 128, 4, 2, 2>(), lds64 = lds_of<64, 64, 4, 2, 2>();
     static_assert(lds <= 64 * 1024, "no attribute needed");
-    if (aligned) {
-        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, true, 8>), grid, dim3(256), lds, st, p);
-        else hipLaunchKernelGGL((linear_bwd_kernel<T, true, 1>), grid, dim3(256), lds, st, p);
+    if (plan.tile == 128) {
+        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, 128, 8>), grid, dim3(256), lds, st, p);
+        else hipLaunchKernelGGL((linear_bwd_kernel<T, 128, 1>), grid, dim3(256), lds, st, p);
     } else {
-        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, false, 8>), grid, dim3(256), lds, st, p);
-        else hipLaunchKernelGGL((linear_bwd_kernel<T, false, 1>), grid, dim3(256), lds, st, p);
+        if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, 64, 8>), grid, dim3(256), lds64, st, p);
+        else hipLaunchKernelGGL((linear_bwd_kernel<T, 64, 1>), grid, dim3(256), lds64, st, p);
     }
     auto join_blocks = [](const LinP& q) { return q.splits > 1 ? (int)(((long long)q.R * up(q.C, 8) + 255) / 256) : 0; };
     const int jw = join_blocks(p.w), jx = a->dx ? join_blocks(p.x) : 0, jd = a->db ? up(N, 16) : 0;
@@ -838,10 +1021,10 @@ extern "C" int dig_linear_act_ws(int M, int N, int K, int dtype) {
     (void)fwd_plan(M, N, K, dtype, s);
     return s > 1 ? (int)((long long)s * M * N) : 0;
 }
-extern "C" int dig_linear_act_bwd_ws(int M, int N, int K, int dtype) {
+extern "C" int dig_linear_act_bwd_ws(int M, int N, int K, int dtype, int dx) {
     if (!shape_ok(M, N, K) || !shape_ok(N, K, 1)) return DIG_EINVAL;
     long long xf;
-    const long long n = bwd_part(M, N, K, dtype, xf) + (long long)dz_chunks(M) * N;
+    const long long n = sum_floats(M, N) + part_floats(bwd_plan(M, N, K, dtype, dx != 0), M, N, K, dx != 0, xf);
     return n < (1ll << 31) ? (int)n : DIG_EINVAL;
 }
 

@@ -1,5 +1,7 @@
 """Thin tensor-level wrappers over the C-ABI kernels (dig_amd/_lib.py).  Activations are NHWC torch tensors
 ([B,H,W,C], bf16 or fp32) living on the HIP device; torch is used only to own memory and streams."""
+import functools
+
 import torch
 
 from . import _lib
@@ -313,6 +315,11 @@ def _gn_check(who, x, gamma, beta, groups, ss, ss_off):
     return B, C, x.numel() // max(1, B * C)
 
 
+@functools.lru_cache(maxsize=1024)
+def _gn_ws(P, C, groups, bwd):
+    return _lib.lib().dig_gn_act_ws(P, C, groups, bwd)
+
+
 def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off=0, res=None, eps=1e-5, want_stats=False):
     """act(GroupNorm(x) * (1 + scale) + shift) [+ res] of any channels-last tensor x [B, ..., C] (bf16 or fp32; rows of one pitch, e.g.
     a channel slice): Block.norm / scale-shift / act (ddp.py:158-166) where no conv3x3 left its statistics, any group count.
@@ -334,7 +341,7 @@ def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off
     if out.numel() == 0:  # no pixel: the statistics of nothing are mean 0, variance 0
         mr[..., 0], mr[..., 1] = 0.0, eps ** -0.5
         return (out, mr) if want_stats else out
-    ws = torch.empty(B * _lib.lib().dig_gn_act_ws(P, C, groups, 0), dtype=torch.float32, device=x.device)
+    ws = torch.empty(B * _gn_ws(P, C, groups, 0), dtype=torch.float32, device=x.device)
     call("gn_act", x=x, gamma=gamma, beta=beta, ss=ss, res=res, out=out, mean_rstd=mr, ws=ws, x_bs=x_bs, x_ld=x_ld, res_bs=r_bs, res_ld=r_ld,
          B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code, dtype=dtype_code(x.dtype), eps=float(eps))
     return (out, mr) if want_stats else out
@@ -364,6 +371,19 @@ def _linear_like(who, name, t, x, N):
     return _row_strides(t, who, name, lead=0)[1]
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_ws(M, N, K, dt):
+    return _lib.lib().dig_linear_act_ws(M, N, K, dt)
+
+
+def _packed(t, rows, K, ld):
+    """Workspace for the 16-byte aligned copy of an operand [rows, K] that the kernels cannot read as it lies, or None."""
+    e = 16 // t.element_size()
+    if K % e == 0 and ld % e == 0 and t.data_ptr() % 16 == 0 and ld * 256 * t.element_size() < 1 << 31:
+        return None
+    return torch.empty(rows, (K + e - 1) // e * e, dtype=t.dtype, device=t.device)
+
+
 def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
     """act(x w^T + bias) [+ res]: nn.Linear or a 1x1 convolution of a channels-last tensor, with what follows it, in one launch.
     x [..., K] (bf16 or fp32; rows of one pitch, e.g. a channel slice), w [N, K] of x's type, bias [N] fp32, act: none | relu | gelu | silu,
@@ -377,7 +397,11 @@ def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
     pre = torch.empty_like(y) if want_pre else None
     if M:
         dt = dtype_code(x.dtype)
-        n = _lib.lib().dig_linear_act_ws(M, N, K, dt)
-        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
-        call("linear_act", x=x, w=w, bias=bias, res=res, out=y, pre=pre, ws=ws, ldx=ldx, ldw=w.stride(0), ldr=ldr, M=M, N=N, K=K, act=code, dtype=dt)
+        n = _linear_ws(M, N, K, dt)
+        if n < 0:
+            raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
+        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
+        ldw = w.stride(0)
+        call("linear_act", x=x, w=w, bias=bias, res=res, out=y, pre=pre, xpack=_packed(x, M, K, ldx), wpack=_packed(w, N, K, ldw), ws=ws, ldx=ldx, ldw=ldw,
+             ldr=ldr, M=M, N=N, K=K, act=code, dtype=dt)
     return (y, pre) if want_pre else y

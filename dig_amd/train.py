@@ -16,6 +16,7 @@ detached), loss_rcams_consistency (through the attention roll-up of all twelve l
 the tape of dig_amd/train_lfca.py).
 torch allocates, copies and reshapes; every arithmetic operation is a C-ABI launch.  There is no CPU fallback.
 """
+import functools
 import math
 
 import torch
@@ -116,11 +117,16 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     dss = torch.empty(B, 2 * C, dtype=F32, device=dev) if ss is not None else None
     if dx.numel() == 0:
         return dx, gb[0].zero_(), gb[1].zero_(), dss.zero_() if dss is not None else None
-    ws = torch.empty(B * lib().dig_gn_act_ws(P, C, groups, 1), dtype=F32, device=dev)
+    ws = torch.empty(B * ops._gn_ws(P, C, groups, 1), dtype=F32, device=dev)
     call("gn_act_bwd", x=x, dy=dy, mean_rstd=mean_rstd, gamma=gamma, beta=beta, ss=ss, dx=dx, dgamma=gb[0], dbeta=gb[1], dss=dss, ws=ws, x_bs=x_bs,
          x_ld=x_ld, dy_bs=d_bs, dy_ld=d_ld, B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code,
          dtype=dtype_code(x.dtype))
     return dx, gb[0], gb[1], dss
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_bwd_ws(M, N, K, dt, dx):
+    return lib().dig_linear_act_bwd_ws(M, N, K, dt, dx)
 
 
 def linear_act_bwd(x, w, dy, pre=None, act="none", need_dx=True, has_bias=True, dw_f32=False):
@@ -140,11 +146,18 @@ def linear_act_bwd(x, w, dy, pre=None, act="none", need_dx=True, has_bias=True, 
     db = torch.empty(N, dtype=F32, device=dev) if has_bias else None
     if M == 0:
         return dx, dw.zero_(), db.zero_() if has_bias else None
-    copy = code or (K % 8 == 0 and (N % 8 or ldy % 8 or dy.data_ptr() % 16))  # dz of its own, rows padded to 8 values
-    dz = torch.empty(M, (N + 7) // 8 * 8, dtype=x.dtype, device=dev) if copy else None
-    ws = torch.empty(lib().dig_linear_act_bwd_ws(M, N, K, dt), dtype=F32, device=dev)
-    call("linear_act_bwd", x=x, w=w, dy=dy, pre=pre if code else None, dx=dx, dw=dw, db=db, dz=dz, ws=ws, ldx=ldx, ldw=w.stride(0), ldy=ldy, ldpre=ldpre,
-         M=M, N=N, K=K, act=code, dtype=dt, dw_f32=int(dw_f32))
+    e = 16 // x.element_size()
+    # dz of its own with an activation, and where the rows of dy do not lie on 16 bytes
+    own_dz = code or N % e or ldy % e or dy.data_ptr() % 16 or ldy * 256 * x.element_size() >= 1 << 31
+    dz = torch.empty(M, (N + 7) // 8 * 8, dtype=x.dtype, device=dev) if own_dz else None
+    n = _linear_bwd_ws(M, N, K, dt, int(need_dx))
+    if n < 0:
+        raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
+    ws = torch.empty(n, dtype=F32, device=dev)
+    ldw = w.stride(0)
+    call("linear_act_bwd", x=x, w=w, dy=dy, pre=pre if code else None, dx=dx, dw=dw, db=db, dz=dz, xpack=ops._packed(x, M, K, ldx),
+         wpack=ops._packed(w, N, K, ldw) if need_dx else None, ws=ws, ldx=ldx, ldw=ldw, ldy=ldy, ldpre=ldpre, M=M, N=N, K=K, act=code, dtype=dt,
+         dw_f32=int(dw_f32))
     return dx, dw, db
 
 

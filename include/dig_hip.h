@@ -855,8 +855,9 @@ int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream);
  * mctformer.py:89-93,163-164; ddp.py:180,194), in a form that can be trained:
  *   pre = x w^T + bias,  out = act(pre) [+ res]
  * x [M][K] row pitch ldx, w [N][K] row pitch ldw, res [M][N] row pitch ldr (elements); bias [N] fp32 or NULL; out, pre [M][N]
- * contiguous (pre NULL: not kept); act: DIG_ACT_*.  Any M, N, K, pitch and alignment; operands whose rows are 16-byte aligned, with K a
- * multiple of 8 (fp32: 4), take the asynchronous path.  ws: dig_linear_act_ws(...) floats (may be NULL when that is 0). */
+ * contiguous (pre NULL: not kept); act: DIG_ACT_*.  Any M, N, K, pitch and alignment.  An operand whose rows do not lie on 16 bytes (its pointer, its
+ * pitch, or K not a multiple of 8 - fp32: 4) or whose pitch reaches 2^31 / 256 bytes is copied to xpack [M][Kp] / wpack [N][Kp] first, Kp = K rounded
+ * up to 16 bytes; otherwise xpack / wpack may be NULL.  ws: dig_linear_act_ws(...) floats (may be NULL when that is 0). */
 typedef struct {
     const void* x;
     const void* w;
@@ -864,6 +865,8 @@ typedef struct {
     const void* res;
     void* out;
     void* pre;
+    void* xpack;
+    void* wpack;
     float* ws;
     long long ldx, ldw, ldr;
     int M, N, K, act, dtype;
@@ -872,8 +875,8 @@ int dig_linear_act(const dig_linear_act_args* a, void* stream);
 int dig_linear_act_ws(int M, int N, int K, int dtype);
 
 /* adjoint: dz = dy * act'(pre),  dx = dz w (NULL: not wanted),  dw = dz^T x (dtype, or fp32 if dw_f32),  db = column sums of dz, fp32
- * (NULL: no bias); all outputs contiguous.  dz: [M][N rounded up to 8] of dtype, workspace; may be NULL when act is DIG_ACT_NONE (dy is then
- * multiplied as it lies; with dz given it is copied there first, which aligns it).  ws: dig_linear_act_bwd_ws(...) floats.
+ * (NULL: no bias); all outputs contiguous.  dz: [M][N rounded up to 8] of dtype, workspace; may be NULL when act is DIG_ACT_NONE and the rows of dy
+ * lie on 16 bytes with N a multiple of 8 (fp32: 4) values (dy is then multiplied as it lies).  xpack, wpack as above.  ws: dig_linear_act_bwd_ws(...) floats.
  * The residual's gradient is dy itself. */
 typedef struct {
     const void* x;
@@ -884,12 +887,14 @@ typedef struct {
     void* dw;
     float* db;
     void* dz;
+    void* xpack;
+    void* wpack;
     float* ws;
     long long ldx, ldw, ldy, ldpre;
     int M, N, K, act, dtype, dw_f32;
 } dig_linear_act_bwd_args;
 int dig_linear_act_bwd(const dig_linear_act_bwd_args* a, void* stream);
-int dig_linear_act_bwd_ws(int M, int N, int K, int dtype);
+int dig_linear_act_bwd_ws(int M, int N, int K, int dtype, int dx);
 
 #ifdef __cplusplus
 }

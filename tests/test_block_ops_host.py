@@ -126,7 +126,7 @@ def test_linear_act_bwd_refusals():
 
 def test_linear_act_c_entry_refuses():
     L = _lib.lib()
-    for fn, optional in (("linear_act", ("bias", "res", "pre")), ("linear_act_bwd", ("pre", "dx", "db", "dz"))):
+    for fn, optional in (("linear_act", ("bias", "res", "pre", "xpack", "wpack")), ("linear_act_bwd", ("pre", "dx", "db", "dz", "xpack", "wpack"))):
         S = _lib.STRUCTS[f"dig_{fn}_args"]
         f = getattr(L, f"dig_{fn}")
         a = S()
@@ -148,4 +148,11 @@ def test_linear_act_c_entry_refuses():
         else:  # a shape whose k is split needs the workspace
             a.ws, a.M, a.N, a.K = None, 16, 64, 8192
             assert L.dig_linear_act_ws(16, 64, 8192, 0) > 0 and f(ctypes.byref(a), None) == -1 and b"needs a workspace" in L.dig_last_error()
-    assert L.dig_linear_act_ws(0, 8, 8, 0) < 0 and L.dig_linear_act_bwd_ws(4, 0, 8, 0) < 0
+            a.ws, a.M, a.N, a.K, a.ldx, a.ldw = 16, 4096, 512, 101, 101, 101  # rows that do not lie on 16 bytes, and no place to pack them
+            assert f(ctypes.byref(a), None) == -2 and b"need xpack" in L.dig_last_error()
+        if fn == "linear_act_bwd":
+            a.act, a.K, a.ldx, a.ldw, a.ldy, a.N = 0, 16, 16, 16, 9, 9
+            assert f(ctypes.byref(a), None) == -2 and b"need dz" in L.dig_last_error()
+            a.ldx = 17
+            assert f(ctypes.byref(a), None) == -2 and b"need xpack" in L.dig_last_error()
+    assert L.dig_linear_act_ws(0, 8, 8, 0) < 0 and L.dig_linear_act_bwd_ws(4, 0, 8, 0, 1) < 0
