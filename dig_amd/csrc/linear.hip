@@ -235,23 +235,33 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
             SQ::piece((wave + j * NW) * 1024 + lane * 16, x, qk[j]);
             qoff[j] = (TQ ? (unsigned)qk[j] * (unsigned)p.ldq + min(x, p.cpad - E - c0) : (unsigned)min(x, p.C - 1 - c0) * (unsigned)p.ldq + qk[j]) * (unsigned)sizeof(T);
         }
+        // Order of the k tiles: a partial one at the end of k goes first, with its pieces past the end replaced by zeros; the whole ones follow from the
+        // corner on.  So the loop fetches without a mask, from a scalar base that moves along and a fixed offset per lane.  What it
+        // fetches behind the last tile is the last whole one again (or, if there is none, pieces that exist) and is not used.
+        const int whole = (kend - kbeg) / BK, rem = (kend - kbeg) % BK;
         const size_t pstep = (TP ? (size_t)BK * p.ldp : (size_t)BK) * sizeof(T), qstep = (TQ ? (size_t)BK * p.ldq : (size_t)BK) * sizeof(T);
-        const char *pb = (const char*)P, *qb = (const char*)Q;  // k tiles are issued in order: the corners move along
-        int left = kend - kbeg;                                 // k values from the next tile to issue on
-        // where the j-th of the wave's PN + QN chunks comes from; past the end of k, also behind the last tile, from zeros
-        auto source = [&](int j) {
-            const bool is_p = j < PN;
-            const int i = is_p ? j : j - PN;
-            const char* src = is_p ? pb + poff[is_p ? i : 0] : qb + qoff[is_p ? 0 : i];
-            return (is_p ? pk[is_p ? i : 0] : qk[is_p ? 0 : i]) < left ? src : (const char*)&zero_piece;
+        const char *pb = (const char*)P, *qb = (const char*)Q;
+        int todo = whole;
+        auto advance = [&]() {
+            todo--;
+            pb += todo > 0 ? pstep : 0;
+            qb += todo > 0 ? qstep : 0;
+        };
+        if (whole == 0) {
+#pragma unroll
+            for (int j = 0; j < PN; j++)
+                if (pk[j] >= rem) poff[j] = 0;
+#pragma unroll
+            for (int j = 0; j < QN; j++)
+                if (qk[j] >= rem) qoff[j] = 0;
+        }
+        auto source = [&](int j) { return j < PN ? pb + poff[j < PN ? j : 0] : qb + qoff[j < PN ? 0 : j - PN]; };
+        auto tail_source = [&](int j) {
+            const char* src = j < PN ? (const char*)P + whole * pstep + poff[j < PN ? j : 0] : (const char*)Q + whole * qstep + qoff[j < PN ? 0 : j - PN];
+            return (j < PN ? pk[j < PN ? j : 0] : qk[j < PN ? 0 : j - PN]) < rem ? src : (const char*)&zero_piece;
         };
         auto place1 = [&](int j, unsigned char* st) { return st + (j < PN ? 0 : SP::BYTES) + (wave + (j < PN ? j : j - PN) * NW) * 1024; };
-        auto issue1 = [&](int j, unsigned char* st) { __builtin_amdgcn_global_load_lds((glb_void*)source(j), (lds_void*)place1(j, st), 16, 0, 0); };
-        auto advance = [&]() {
-            pb += pstep;
-            qb += qstep;
-            left -= BK;
-        };
+        auto dma = [&](const char* src, int j, unsigned char* st) { __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)place1(j, st), 16, 0, 0); };
         f32x4 rg[STAGED ? PN + QN : 1];
         auto fetch = [&]() {  // a tile into registers
 #pragma unroll
@@ -261,7 +271,12 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
         auto put1 = [&](int j, unsigned char* st) { *reinterpret_cast<f32x4*>(place1(j, st) + lane * 16) = rg[STAGED ? j : 0]; };
         F fp[2][TRN], fq[2][TCN];
         if constexpr (STAGED) {
-            fetch();
+            if (rem) {
+#pragma unroll
+                for (int j = 0; j < PN + QN; j++) rg[STAGED ? j : 0] = *reinterpret_cast<const f32x4*>(tail_source(j));
+            } else {
+                fetch();
+            }
 #pragma unroll
             for (int j = 0; j < PN + QN; j++) put1(j, smem);
             fetch();
@@ -269,9 +284,14 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
         } else {
 #pragma unroll
             for (int i = 0; i < NS; i++) {
+                if (i == 0 && rem) {
 #pragma unroll
-                for (int j = 0; j < PN + QN; j++) issue1(j, smem + i * STAGE);
-                advance();
+                    for (int j = 0; j < PN + QN; j++) dma(tail_source(j), j, smem);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PN + QN; j++) dma(source(j), j, smem + i * STAGE);
+                    advance();
+                }
             }
             dma_wait_barrier<(NS - 1) * (PN + QN)>();
         }
@@ -279,9 +299,8 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
         for (int j = 0; j < TCN; j++) fq[0][j] = qfrag(smem, j, 0);
 #pragma unroll
         for (int i = 0; i < TRN; i++) fp[0][i] = pfrag(smem, i, 0);
-        unsigned char *cur = smem, *nxt = smem + STAGE;
-        // one copy of the matrix instructions and no branch in it: behind the last tile, tiles of zeros are fetched and not used
-        for (int kt = 0; kt < nk; kt++) {
+        // one copy of the matrix instructions per place in LDS and no branch in it
+        auto tile = [&](unsigned char* cur, unsigned char* nxt) {
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 const unsigned char* from = kk ? nxt : cur;
@@ -312,14 +331,27 @@ __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctile
                         }
                     } else if (kk == 1) {  // a few at a time: a burst of them stalls the wave
 #pragma unroll
-                        for (int e = i * (PN + QN) / TRN; e < (i + 1) * (PN + QN) / TRN; e++) issue1(e, cur);
+                        for (int e = i * (PN + QN) / TRN; e < (i + 1) * (PN + QN) / TRN; e++) dma(source(e), e, cur);
                         if (i == TRN - 1) advance();
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            cur = nxt;
-            nxt = cur == smem + (NS - 1) * STAGE ? smem : cur + STAGE;
+        };
+        if constexpr (NS == 2) {
+            for (int kt = 0;;) {
+                tile(smem, smem + STAGE);
+                if (++kt >= nk) break;
+                tile(smem + STAGE, smem);
+                if (++kt >= nk) break;
+            }
+        } else {
+            unsigned char *cur = smem, *nxt = smem + STAGE;
+            for (int kt = 0; kt < nk; kt++) {
+                tile(cur, nxt);
+                cur = nxt;
+                nxt = cur == smem + (NS - 1) * STAGE ? smem : cur + STAGE;
+            }
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the last of them have landed before LDS is used again
     }
