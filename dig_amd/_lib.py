@@ -164,6 +164,30 @@ def call(fn, stream=None, **kw):
         tr(fn, kw, 1)
 
 
+def launch(fn, dev, *vals):
+    """Launch dig_<fn> with its argument block's values in field order (pointers as integers, 0 = NULL), for wrappers that have checked their
+    tensors already: they live on HIP device number `dev`.  The stream is that device's current one."""
+    import torch
+
+    e = _ENTRIES.get(fn)
+    if e is None:
+        e = _ENTRIES[fn] = _Entry(fn)
+    block = e.pack(*vals)
+    tr = TRACE
+    if tr is not None:
+        kw = dict(zip(e.slot, vals))
+        tr(fn, kw, 0)
+    if dev == torch._C._cuda_getDevice():
+        rc = e.func(block, torch._C._cuda_getCurrentRawStream(dev))
+    else:  # the launchers key their per-device state on hipGetDevice()
+        with torch.cuda.device(dev):
+            rc = e.func(block, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        raise RuntimeError(f"dig_{fn} failed ({rc}): {lib().dig_last_error().decode()}")
+    if tr is not None:
+        tr(fn, kw, 1)
+
+
 def dtype_code(torch_dtype):
     import torch
 

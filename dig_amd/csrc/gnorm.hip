@@ -1040,10 +1040,14 @@ bool read_once(long long bytes) { return bytes > (128ll << 20); }
 constexpr int SLAB_BT = 512;
 constexpr int SLAB_MAX = 512 << 10;  // bytes of x that one block of the backward reads twice
 
+// whether the one-block forms take a shape of n vectors per thread
+bool fwd_one_block(int n, int esize) { return n > 0 && n <= (esize == 2 ? 32 : 16); }
+bool bwd_one_block(int n, int P, const BGeo& g, int esize) { return n > 0 && (n <= (esize == 2 ? 16 : 8) || (long long)P * g.LP * 8 * esize <= SLAB_MAX); }
+
 template <typename T, int ACT> int fwd_launch_vec(const FwdP& p, int B, hipStream_t st, bool& done) {
     BGeo g;
     const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
-    done = n > 0 && n <= (sizeof(T) == 2 ? 32 : 16);
+    done = fwd_one_block(n, (int)sizeof(T));
     if (!done) return DIG_OK;
     DIG_CHECK((long long)B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
     const dim3 grid((unsigned)(B * g.nch));
@@ -1091,7 +1095,7 @@ template <typename T, int ACT> int bwd_launch_vec(BwdP p, hipStream_t st, bool& 
     BGeo g;
     const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
     const int most = sizeof(T) == 2 ? 16 : 8;
-    done = n > 0 && (n <= most || (long long)p.q.P * g.LP * 8 * (long long)sizeof(T) <= SLAB_MAX);
+    done = bwd_one_block(n, p.q.P, g, (int)sizeof(T));
     if (!done) return DIG_OK;
     DIG_CHECK((long long)p.B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
     const dim3 grid((unsigned)(p.B * g.nch));
@@ -1151,19 +1155,17 @@ bool shape_ok(int B, int P, int C, int G) { return B > 0 && P > 0 && C > 0 && G 
 
 }  // namespace
 
-extern "C" int dig_gn_act_ws(int P, int C, int groups, int bwd) {
-    if (!shape_ok(1, P, C, groups)) return DIG_EINVAL;
-    int most = 0;
-    for (int vec = 0; vec < 2; vec++) {  // whichever of the two the strides and the alignment will select
-        const Geo q = geo_any(P, C, groups, vec != 0);
-        const int n = (bwd ? q.S * C * 2 + groups * 2 : 0) + groups * q.nch * q.S * 2;
-        most = n > most ? n : most;
-    }
-    return most;
+extern "C" int dig_gn_act_ws(int P, int C, int groups, int bwd, int vec, int dtype) {
+    if (!shape_ok(1, P, C, groups) || (vec && C % 8)) return DIG_EINVAL;
+    BGeo g;
+    const int esize = dtype == DIG_BF16 ? 2 : 4;
+    if (vec && (bwd ? bwd_one_block(block_geo(P, C, groups, esize, g), P, g, esize) : fwd_one_block(block_geo(P, C, groups, esize, g), esize))) return bwd ? C * 2 : 0;
+    const Geo q = geo_any(P, C, groups, vec != 0);
+    return (bwd ? q.S * C * 2 + groups * 2 : 0) + groups * q.nch * q.S * 2;
 }
 
 extern "C" int dig_gn_act(const dig_gn_act_args* a, void* stream) {
-    DIG_CHECK(a && a->x && a->gamma && a->beta && a->out && a->mean_rstd && a->ws, DIG_EINVAL, "gn_act: null pointer");
+    DIG_CHECK(a && a->x && a->gamma && a->beta && a->out && a->mean_rstd, DIG_EINVAL, "gn_act: null pointer");
     DIG_CHECK(shape_ok(a->B, a->P, a->C, a->groups), DIG_EINVAL, "gn_act: bad shape B=%d P=%d C=%d groups=%d", a->B, a->P, a->C, a->groups);
     DIG_CHECK(a->act >= 0 && a->act <= 3, DIG_EINVAL, "gn_act: act %d", a->act);
     DIG_CHECK(a->dtype == DIG_BF16 || a->dtype == DIG_F32, DIG_EINVAL, "gn_act: dtype %d", a->dtype);
@@ -1173,6 +1175,7 @@ extern "C" int dig_gn_act(const dig_gn_act_args* a, void* stream) {
                      (!a->res || (a->res_bs % 8 == 0 && a->res_ld % 8 == 0 && aligned16(a->res)));
     FwdP p{a->x, a->gamma, a->beta, a->ss, a->res, a->out, a->mean_rstd, a->ws, a->x_bs, a->x_ld, a->res_bs, a->res_ld, a->ss_ld, a->ss_off, wide_params(a->gamma, a->beta, a->ss, a->ss_ld, a->ss_off, a->C), a->eps, geo_any(a->P, a->C, a->groups, vec)};
     DIG_CHECK((long long)a->B * p.q.nch * p.q.S < (1ll << 31) && (long long)a->B * a->groups < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
+    DIG_CHECK(a->ws || dig_gn_act_ws(a->P, a->C, a->groups, 0, vec, a->dtype) == 0, DIG_EINVAL, "gn_act: this shape needs a workspace");
     hipStream_t st = (hipStream_t)stream;
     if (a->dtype == DIG_BF16) return vec ? fwd_act<bf16, 8>(p, a->B, a->act, st) : fwd_act<bf16, 1>(p, a->B, a->act, st);
     return vec ? fwd_act<float, 8>(p, a->B, a->act, st) : fwd_act<float, 1>(p, a->B, a->act, st);

@@ -261,63 +261,83 @@ def bilinear_ac_into(x, out, c_off):
 
 
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_F32 = torch.float32
+_DT = {torch.bfloat16: _lib.DIG_BF16, torch.float32: _lib.DIG_F32}
 
 
 def _act_code(act, who):
-    if act not in ACTS:
+    code = ACTS.get(act)
+    if code is None:
         raise ValueError(f"{who}: act must be one of {sorted(ACTS)}, got {act!r}")
-    return ACTS[act]
+    return code
 
 
 def _on_device(who, dev, **tensors):
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{who}: {name} lives on {t.device} but x on {dev}")
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"{who}: {name} lives on {t.device} but x on cuda:{dev}")
 
 
-def _f32_vec(who, name, t, n):
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+def _f32_vec(who, name, t, n, dev):
+    if t.get_device() != dev:
+        _on_device(who, dev, **{name: t})
+    if t.dtype is not _F32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous float32 tensor of {n} values, got {t.dtype} {tuple(t.shape)}")
 
 
 def _row_strides(t, who, name, lead=1):
     """Element strides (outer, row) of a channels-last tensor [d0, ..., C] whose leading dimensions from `lead` on step through rows
     of one pitch (lead = 1: [B, rows, C]; lead = 0: [rows, C] and outer is 0).  Slices of the channels or of the images qualify."""
-    if t.dim() < lead + 1:
-        raise ValueError(f"{who}: {name} needs at least {lead + 1} dimensions, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape = t.shape
+    if len(shape) < lead + 1:
+        raise ValueError(f"{who}: {name} needs at least {lead + 1} dimensions, got {tuple(shape)}")
+    if t.is_contiguous():
+        return (t.stride(0) if lead and shape[0] > 1 else 0), shape[-1]
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{who}: the channels of {name} must be adjacent in memory (strides {t.stride()})")
-    dims = [(t.shape[i], t.stride(i)) for i in range(lead, t.dim() - 1) if t.shape[i] != 1]
+    dims = [(shape[i], t.stride(i)) for i in range(lead, len(shape) - 1) if shape[i] != 1]
     for (_, outer), (n, inner) in zip(dims, dims[1:]):
         if outer != n * inner:
-            raise ValueError(f"{who}: the rows of {name} must have one pitch (shape {tuple(t.shape)}, strides {t.stride()})")
-    ld = dims[-1][1] if dims else t.shape[-1]
-    return (t.stride(0) if lead and t.shape[0] > 1 else 0), ld
+            raise ValueError(f"{who}: the rows of {name} must have one pitch (shape {tuple(shape)}, strides {t.stride()})")
+    ld = dims[-1][1] if dims else shape[-1]
+    return (t.stride(0) if lead and shape[0] > 1 else 0), ld
+
+
+def _storage_code(who, t):
+    code = _DT.get(t.dtype)
+    return dtype_code(t.dtype) if code is None else code
 
 
 def _gn_check(who, x, gamma, beta, groups, ss, ss_off):
-    if not x.is_cuda:
+    """-> (device number, B, C, pixels, storage type)"""
+    dev = x.get_device()
+    if dev < 0:
         raise RuntimeError(f"{who} runs on the HIP device only (no CPU fallback): x is on {x.device}")
-    if x.dim() < 2:
-        raise ValueError(f"{who}: x must be [B, ..., C], got {tuple(x.shape)}")
-    dtype_code(x.dtype)
-    B, C = x.shape[0], x.shape[-1]
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{who}: x must be [B, ..., C], got {tuple(shape)}")
+    dt = _storage_code(who, x)
+    B, C = shape[0], shape[-1]
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"{who}: {C} channels do not divide into {groups} groups")
-    _on_device(who, x.device, gamma=gamma, beta=beta, ss=ss)
-    _f32_vec(who, "gamma", gamma, C)
-    _f32_vec(who, "beta", beta, C)
+    _f32_vec(who, "gamma", gamma, C, dev)
+    _f32_vec(who, "beta", beta, C, dev)
     if ss is not None:
-        if ss.dtype != torch.float32 or ss.dim() != 2 or ss.shape[0] != B or ss.stride(1) != 1:
+        if ss.get_device() != dev:
+            _on_device(who, dev, ss=ss)
+        if ss.dtype is not _F32 or ss.dim() != 2 or ss.shape[0] != B or ss.stride(1) != 1:
             raise ValueError(f"{who}: ss must be float32 rows [B, ld] of (scale | shift), got {ss.dtype} {tuple(ss.shape)}")
         if ss_off < 0 or ss.shape[1] < ss_off + 2 * C:
             raise ValueError(f"{who}: ss rows of {ss.shape[1]} values do not hold scale and shift of {C} channels at {ss_off}")
-    return B, C, x.numel() // max(1, B * C)
+    P = 1
+    for n in shape[1:-1]:
+        P *= n
+    return dev, B, C, P, dt
 
 
 @functools.lru_cache(maxsize=1024)
-def _gn_ws(P, C, groups, bwd):
-    return _lib.lib().dig_gn_act_ws(P, C, groups, bwd)
+def _gn_ws(P, C, groups, bwd, vec, dt):
+    return _lib.lib().dig_gn_act_ws(P, C, groups, bwd, vec, dt)
 
 
 def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off=0, res=None, eps=1e-5, want_stats=False):
@@ -326,47 +346,61 @@ def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off
     gamma, beta [C] fp32; ss [B, ld] fp32 rows holding (scale | shift) at ss_off; act: none | relu | gelu | silu; res like x.
     -> y contiguous, in x's type; with want_stats (y, mean_rstd [B, groups, 2] fp32), which train.group_norm_act_bwd takes."""
     who = "group_norm_act"
-    B, C, P = _gn_check(who, x, gamma, beta, groups, ss, ss_off)
+    dev, B, C, P, dt = _gn_check(who, x, gamma, beta, groups, ss, ss_off)
     code = _act_code(act, who)
     if not eps > 0:
         raise ValueError(f"{who}: eps must be positive, got {eps}")
+    x_bs, x_ld = _row_strides(x, who, "x")
+    r_bs = r_ld = rp = 0
     if res is not None:
-        _on_device(who, x.device, res=res)
+        if res.get_device() != dev:
+            _on_device(who, dev, res=res)
         if res.shape != x.shape or res.dtype != x.dtype:
             raise ValueError(f"{who}: res must be like x ({x.dtype} {tuple(x.shape)}), got {res.dtype} {tuple(res.shape)}")
-    x_bs, x_ld = _row_strides(x, who, "x")
-    r_bs, r_ld = _row_strides(res, who, "res") if res is not None else (0, 0)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mr = torch.empty(B, groups, 2, dtype=torch.float32, device=x.device)
-    if out.numel() == 0:  # no pixel: the statistics of nothing are mean 0, variance 0
+        r_bs, r_ld = _row_strides(res, who, "res")
+        rp = res.data_ptr()
+    out, mr = x.new_empty(x.shape), gamma.new_empty((B, groups, 2))
+    if B * P == 0:  # no pixel: the statistics of nothing are mean 0, variance 0
         mr[..., 0], mr[..., 1] = 0.0, eps ** -0.5
         return (out, mr) if want_stats else out
-    ws = torch.empty(B * _gn_ws(P, C, groups, 0), dtype=torch.float32, device=x.device)
-    call("gn_act", x=x, gamma=gamma, beta=beta, ss=ss, res=res, out=out, mean_rstd=mr, ws=ws, x_bs=x_bs, x_ld=x_ld, res_bs=r_bs, res_ld=r_ld,
-         B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code, dtype=dtype_code(x.dtype), eps=float(eps))
+    xp, op = x.data_ptr(), out.data_ptr()
+    vec = not (C % 8 or (x_bs | x_ld | r_bs | r_ld) % 8 or (xp | op | rp) % 16)
+    n = _gn_ws(P, C, groups, 0, vec, dt)
+    ws = gamma.new_empty(B * n) if n else None
+    _lib.launch("gn_act", dev, xp, gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, rp, op, mr.data_ptr(), ws.data_ptr() if n else 0,
+                x_bs, x_ld, r_bs, r_ld, B, P, C, groups, ss.stride(0) if ss is not None else 0, ss_off, code, dt, eps)
     return (out, mr) if want_stats else out
 
 
 def _linear_check(who, x, w, bias):
-    if not x.is_cuda:
+    """-> (device number, M, N, K, storage type)"""
+    dev = x.get_device()
+    if dev < 0:
         raise RuntimeError(f"{who} runs on the HIP device only (no CPU fallback): x is on {x.device}")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or w.numel() == 0:
-        raise ValueError(f"{who}: x [..., K] and w [N, K] do not fit: {tuple(x.shape)}, {tuple(w.shape)}")
-    dtype_code(x.dtype)
+    xs, wsh = x.shape, w.shape
+    if len(xs) < 1 or len(wsh) != 2 or xs[-1] != wsh[1] or not (wsh[0] and wsh[1]):
+        raise ValueError(f"{who}: x [..., K] and w [N, K] do not fit: {tuple(xs)}, {tuple(wsh)}")
+    dt = _storage_code(who, x)
     if w.dtype != x.dtype:
         raise ValueError(f"{who}: x is {x.dtype} but w {w.dtype}")
-    _on_device(who, x.device, w=w, bias=bias)
-    N, K = w.shape
+    if w.get_device() != dev:
+        _on_device(who, dev, w=w)
+    N, K = wsh
     if K > 1 and w.stride(1) != 1:
         raise ValueError(f"{who}: the rows of w must lie with K adjacent (strides {w.stride()})")
     if bias is not None:
-        _f32_vec(who, "bias", bias, N)
-    return x.numel() // K, N, K
+        _f32_vec(who, "bias", bias, N, dev)
+    M = 1
+    for n in xs[:-1]:
+        M *= n
+    return dev, M, N, K, dt
 
 
-def _linear_like(who, name, t, x, N):
-    _on_device(who, x.device, **{name: t})
-    if t.shape != (*x.shape[:-1], N) or t.dtype != x.dtype:
+def _linear_like(who, name, t, x, N, dev):
+    """-> the row pitch of t, [..., N] beside x [..., K]"""
+    if t.get_device() != dev:
+        _on_device(who, dev, **{name: t})
+    if t.dtype != x.dtype or t.dim() != x.dim() or t.shape[-1] != N or t.shape[:-1] != x.shape[:-1]:
         raise ValueError(f"{who}: {name} must be {x.dtype} {(*x.shape[:-1], N)}, got {t.dtype} {tuple(t.shape)}")
     return _row_strides(t, who, name, lead=0)[1]
 
@@ -376,12 +410,11 @@ def _linear_ws(M, N, K, dt):
     return _lib.lib().dig_linear_act_ws(M, N, K, dt)
 
 
-def _packed(t, rows, K, ld):
-    """Workspace for the 16-byte aligned copy of an operand [rows, K] that the kernels cannot read as it lies, or None."""
-    e = 16 // t.element_size()
-    if K % e == 0 and ld % e == 0 and t.data_ptr() % 16 == 0 and ld * 256 * t.element_size() < 1 << 31:
+def _packed(t, p, rows, K, ld, e):
+    """Workspace for the 16-byte aligned copy (e values per 16 bytes) of an operand [rows, K] that the kernels cannot read as it lies, or None."""
+    if not (K % e or ld % e or p % 16 or ld * 4096 >= e << 31):
         return None
-    return torch.empty(rows, (K + e - 1) // e * e, dtype=t.dtype, device=t.device)
+    return t.new_empty((rows, (K + e - 1) // e * e))
 
 
 def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
@@ -389,19 +422,20 @@ def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
     x [..., K] (bf16 or fp32; rows of one pitch, e.g. a channel slice), w [N, K] of x's type, bias [N] fp32, act: none | relu | gelu | silu,
     res [..., N].  -> y [..., N]; with want_pre (y, pre = x w^T + bias in x's type), which train.linear_act_bwd takes."""
     who = "linear_act"
-    M, N, K = _linear_check(who, x, w, bias)
+    dev, M, N, K, dt = _linear_check(who, x, w, bias)
     code = _act_code(act, who)
-    ldr = _linear_like(who, "res", res, x, N) if res is not None else 0
+    ldr = _linear_like(who, "res", res, x, N, dev) if res is not None else 0
     ldx = _row_strides(x, who, "x", lead=0)[1]
-    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    pre = torch.empty_like(y) if want_pre else None
+    y = x.new_empty((*x.shape[:-1], N))
+    pre = x.new_empty(y.shape) if want_pre else None
     if M:
-        dt = dtype_code(x.dtype)
         n = _linear_ws(M, N, K, dt)
         if n < 0:
             raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
-        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-        ldw = w.stride(0)
-        call("linear_act", x=x, w=w, bias=bias, res=res, out=y, pre=pre, xpack=_packed(x, M, K, ldx), wpack=_packed(w, N, K, ldw), ws=ws, ldx=ldx, ldw=ldw,
-             ldr=ldr, M=M, N=N, K=K, act=code, dtype=dt)
+        ws = torch.empty(n, dtype=_F32, device=x.device) if n else None
+        xp, wp, ldw, e = x.data_ptr(), w.data_ptr(), w.stride(0), 8 if dt == 0 else 4
+        xk, wk = _packed(x, xp, M, K, ldx, e), _packed(w, wp, N, K, ldw, e)
+        _lib.launch("linear_act", dev, xp, wp, bias.data_ptr() if bias is not None else 0, res.data_ptr() if res is not None else 0, y.data_ptr(),
+                    pre.data_ptr() if want_pre else 0, xk.data_ptr() if xk is not None else 0, wk.data_ptr() if wk is not None else 0, ws.data_ptr() if n else 0,
+                    ldx, ldw, ldr, M, N, K, code, dt)
     return (y, pre) if want_pre else y

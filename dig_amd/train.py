@@ -22,7 +22,7 @@ import math
 import torch
 
 from . import ops
-from ._lib import call, dtype_code, lib
+from ._lib import call, launch, lib
 from .cam import _layernorm, _pack, _pos_embed
 
 F32 = torch.float32
@@ -104,24 +104,27 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     if mean_rstd.dim() != 3 or mean_rstd.shape[2] != 2 or mean_rstd.dtype != F32 or not mean_rstd.is_contiguous() or mean_rstd.shape[0] != x.shape[0]:
         raise ValueError(f"{who}: mean_rstd must be the contiguous float32 [B, groups, 2] of the forward, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
     groups = mean_rstd.shape[1]
-    B, C, P = ops._gn_check(who, x, gamma, beta, groups, ss, ss_off)
+    dev, B, C, P, dt = ops._gn_check(who, x, gamma, beta, groups, ss, ss_off)
     code = ops._act_code(act, who)
-    ops._on_device(who, x.device, mean_rstd=mean_rstd, dy=dy)
+    if mean_rstd.get_device() != dev or dy.get_device() != dev:
+        ops._on_device(who, dev, mean_rstd=mean_rstd, dy=dy)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"{who}: dy must be like x ({x.dtype} {tuple(x.shape)}), got {dy.dtype} {tuple(dy.shape)}")
     x_bs, x_ld = ops._row_strides(x, who, "x")
     d_bs, d_ld = ops._row_strides(dy, who, "dy")
-    dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    gb = torch.empty(2, C, dtype=F32, device=dev)
-    dss = torch.empty(B, 2 * C, dtype=F32, device=dev) if ss is not None else None
-    if dx.numel() == 0:
-        return dx, gb[0].zero_(), gb[1].zero_(), dss.zero_() if dss is not None else None
-    ws = torch.empty(B * ops._gn_ws(P, C, groups, 1), dtype=F32, device=dev)
-    call("gn_act_bwd", x=x, dy=dy, mean_rstd=mean_rstd, gamma=gamma, beta=beta, ss=ss, dx=dx, dgamma=gb[0], dbeta=gb[1], dss=dss, ws=ws, x_bs=x_bs,
-         x_ld=x_ld, dy_bs=d_bs, dy_ld=d_ld, B=B, P=P, C=C, groups=groups, ss_ld=ss.stride(0) if ss is not None else 0, ss_off=ss_off, act=code,
-         dtype=dtype_code(x.dtype))
-    return dx, gb[0], gb[1], dss
+    dx = x.new_empty(x.shape)
+    dgamma, dbeta = gamma.new_empty(C), gamma.new_empty(C)
+    dss = gamma.new_empty((B, 2 * C)) if ss is not None else None
+    if B * P == 0:
+        return dx, dgamma.zero_(), dbeta.zero_(), dss.zero_() if dss is not None else None
+    xp, dp, op = x.data_ptr(), dy.data_ptr(), dx.data_ptr()
+    vec = not (C % 8 or (x_bs | x_ld | d_bs | d_ld) % 8 or (xp | dp | op) % 16)
+    n = ops._gn_ws(P, C, groups, 1, vec, dt)
+    ws = gamma.new_empty(B * n)
+    launch("gn_act_bwd", dev, xp, dp, mean_rstd.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, op, dgamma.data_ptr(),
+           dbeta.data_ptr(), dss.data_ptr() if ss is not None else 0, ws.data_ptr(), x_bs, x_ld, d_bs, d_ld, B, P, C, groups,
+           ss.stride(0) if ss is not None else 0, ss_off, code, dt)
+    return dx, dgamma, dbeta, dss
 
 
 @functools.lru_cache(maxsize=1024)
@@ -133,31 +136,29 @@ def linear_act_bwd(x, w, dy, pre=None, act="none", need_dx=True, has_bias=True, 
     """Adjoint of ops.linear_act for x [..., K], w [N, K], dy [..., N] and, with an activation, the pre it returned
     -> (dx like x or None, dw [N, K] in w's type or fp32, db [N] fp32 or None).  The gradient of the residual is dy itself."""
     who = "linear_act_bwd"
-    M, N, K = ops._linear_check(who, x, w, None)
+    dev, M, N, K, dt = ops._linear_check(who, x, w, None)
     code = ops._act_code(act, who)
-    ldy = ops._linear_like(who, "dy", dy, x, N)
+    ldy = ops._linear_like(who, "dy", dy, x, N, dev)
     if code and pre is None:
         raise ValueError(f"{who}: act={act!r} needs pre, the pre-activation of the forward (want_pre=True)")
-    ldpre = ops._linear_like(who, "pre", pre, x, N) if code else 0
+    ldpre = ops._linear_like(who, "pre", pre, x, N, dev) if code else 0
     ldx = ops._row_strides(x, who, "x", lead=0)[1]
-    dev, dt = x.device, dtype_code(x.dtype)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
-    dw = torch.empty(N, K, dtype=F32 if dw_f32 else w.dtype, device=dev)
-    db = torch.empty(N, dtype=F32, device=dev) if has_bias else None
+    dx = x.new_empty(x.shape) if need_dx else None
+    dw = w.new_empty((N, K), dtype=F32) if dw_f32 else w.new_empty((N, K))
+    db = torch.empty(N, dtype=F32, device=x.device) if has_bias else None
     if M == 0:
         return dx, dw.zero_(), db.zero_() if has_bias else None
-    e = 16 // x.element_size()
-    # dz of its own with an activation, and where the rows of dy do not lie on 16 bytes
-    own_dz = code or N % e or ldy % e or dy.data_ptr() % 16 or ldy * 256 * x.element_size() >= 1 << 31
-    dz = torch.empty(M, (N + 7) // 8 * 8, dtype=x.dtype, device=dev) if own_dz else None
-    n = _linear_bwd_ws(M, N, K, dt, int(need_dx))
+    n = _linear_bwd_ws(M, N, K, dt, need_dx)
     if n < 0:
         raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
-    ws = torch.empty(n, dtype=F32, device=dev)
-    ldw = w.stride(0)
-    call("linear_act_bwd", x=x, w=w, dy=dy, pre=pre if code else None, dx=dx, dw=dw, db=db, dz=dz, xpack=ops._packed(x, M, K, ldx),
-         wpack=ops._packed(w, N, K, ldw) if need_dx else None, ws=ws, ldx=ldx, ldw=ldw, ldy=ldy, ldpre=ldpre, M=M, N=N, K=K, act=code, dtype=dt,
-         dw_f32=int(dw_f32))
+    ws = torch.empty(n, dtype=F32, device=x.device)
+    xp, wp, dp, ldw, e = x.data_ptr(), w.data_ptr(), dy.data_ptr(), w.stride(0), 8 if dt == 0 else 4
+    # dz of its own with an activation, and where the rows of dy do not lie on 16 bytes
+    dz = x.new_empty((M, (N + 7) // 8 * 8)) if code or N % e or ldy % e or dp % 16 or ldy * 4096 >= e << 31 else None
+    xk, wk = ops._packed(x, xp, M, K, ldx, e), ops._packed(w, wp, N, K, ldw, e) if need_dx else None
+    launch("linear_act_bwd", dev, xp, wp, dp, pre.data_ptr() if code else 0, dx.data_ptr() if need_dx else 0, dw.data_ptr(), db.data_ptr() if has_bias else 0,
+           dz.data_ptr() if dz is not None else 0, xk.data_ptr() if xk is not None else 0, wk.data_ptr() if wk is not None else 0, ws.data_ptr(), ldx, ldw, ldy, ldpre,
+           M, N, K, code, dt, int(dw_f32))
     return dx, dw, db
 
 

@@ -809,7 +809,8 @@ int dig_kd_bin_grad(const dig_kd_bin_grad_args* a, void* stream);
  * x [B][P][C] at b * x_bs + p * x_ld + c (element strides), res likewise, out [B][P][C] contiguous; any C, groups with
  * C % groups == 0, any alignment (16-byte aligned rows with C % 8 == 0 take 16-byte accesses).
  *   gamma, beta [C];  ss: per image row b * ss_ld + ss_off: scale [C] | shift [C], or NULL;  act: DIG_ACT_*
- *   mean_rstd [B][groups][2]: written, what the backward needs;  ws: B * dig_gn_act_ws(P, C, groups, 0) floats */
+ *   mean_rstd [B][groups][2]: written, what the backward needs;  ws: B * dig_gn_act_ws(P, C, groups, 0, vec, dtype) floats, NULL
+ *   when that is 0; vec: whether all rows are 16-byte aligned as above */
 #define DIG_ACT_NONE 0
 #define DIG_ACT_RELU 1
 #define DIG_ACT_GELU 2 /* erf form */
@@ -829,10 +830,10 @@ typedef struct {
 } dig_gn_act_args;
 int dig_gn_act(const dig_gn_act_args* a, void* stream);
 /* workspace floats per image of dig_gn_act (bwd = 0) / dig_gn_act_bwd (bwd = 1); negative for a bad shape */
-int dig_gn_act_ws(int P, int C, int groups, int bwd);
+int dig_gn_act_ws(int P, int C, int groups, int bwd, int vec, int dtype);
 
 /* adjoint: x, dy (strided as above), mean_rstd of the forward -> dx [B][P][C] contiguous, dgamma [C], dbeta [C] and, with ss,
- * dss [B][2C] = (dscale | dshift).  The residual's gradient is dy itself.  ws: B * dig_gn_act_ws(P, C, groups, 1) floats */
+ * dss [B][2C] = (dscale | dshift).  The residual's gradient is dy itself.  ws: B * dig_gn_act_ws(P, C, groups, 1, vec, dtype) floats */
 typedef struct {
     const void* x;
     const void* dy;

@@ -22,6 +22,9 @@ class _Fake(torch.Tensor):
     def device(self):
         return torch.device("cuda", 0)
 
+    def get_device(self):
+        return 0
+
 
 def F(*shape, dtype=torch.float32):
     return _Fake(torch.zeros(*shape, dtype=dtype))
@@ -29,11 +32,13 @@ def F(*shape, dtype=torch.float32):
 
 @pytest.fixture(autouse=True)
 def _no_launch(monkeypatch):
-    def refuse(fn, **kw):
+    def refuse(fn, *a, **kw):
         raise AssertionError(f"dig_{fn} would have been launched")
 
     monkeypatch.setattr(ops, "call", refuse)
     monkeypatch.setattr(train, "call", refuse)
+    monkeypatch.setattr(_lib, "launch", refuse)
+    monkeypatch.setattr(train, "launch", refuse)
 
 
 def test_group_norm_act_refusals():
@@ -94,7 +99,11 @@ def test_gn_act_c_entry_refuses():
         if fn == "gn_act":
             a.ss_ld = 31
         assert f(ctypes.byref(a), None) == -1 and b"do not hold" in L.dig_last_error()
-    assert L.dig_gn_act_ws(0, 16, 4, 0) < 0 and L.dig_gn_act_ws(5, 16, 3, 0) < 0 and L.dig_gn_act_ws(5, 16, 4, 1) > 0
+        if fn == "gn_act":  # a shape of several launches needs a workspace
+            a.ss, a.ws, a.P, a.C = None, None, 1 << 20, 64
+            assert f(ctypes.byref(a), None) == -1 and b"needs a workspace" in L.dig_last_error()
+    assert L.dig_gn_act_ws(0, 16, 4, 0, 1, 0) < 0 and L.dig_gn_act_ws(5, 16, 3, 0, 0, 0) < 0 and L.dig_gn_act_ws(5, 12, 3, 0, 1, 0) < 0
+    assert L.dig_gn_act_ws(5, 16, 4, 0, 1, 0) == 0 and L.dig_gn_act_ws(5, 16, 4, 1, 1, 0) > 0 and L.dig_gn_act_ws(5, 16, 4, 0, 0, 0) > 0
 
 
 def test_linear_act_refusals():
