@@ -768,7 +768,7 @@ int fwd_plan(int M, int N, int K, int dtype, int& splits) {
         int br, bc, slots;
         double fill, step, step_f32;
     };
-    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 15.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 7.0}};
+    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 14.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 7.0}};
     const bool f32 = dtype != DIG_BF16;
     const int nk = up(K, f32 ? 32 : 64);
     splits = 1;
@@ -787,7 +787,7 @@ int fwd_plan(int M, int N, int K, int dtype, int& splits) {
         }
     }
     const long long t64 = (long long)up(M, 64) * up(N, 64);
-    if (t64 < 256 && nk >= 16) {
+    if (t64 <= 128 && nk >= 16) {
         int n = (int)(512 / t64);
         if (n > nk / 8) n = nk / 8;
         if (n > 64) n = 64;
