@@ -144,8 +144,10 @@ def call(fn, stream=None, **kw):
             raise TypeError(f"{e.sname} has no field {k!r}")
         i, n = at
         if n:
-            for j, x in enumerate(v):
-                vals[i + j] = x
+            v = tuple(v)
+            if len(v) > n:
+                raise IndexError(f"dig_{fn}: {k!r} holds {n} values, got {len(v)}")
+            vals[i:i + len(v)] = v
         elif v is not None:
             vals[i] = v
     block = e.pack(*vals)
@@ -172,7 +174,10 @@ def launch(fn, dev, *vals):
     e = _ENTRIES.get(fn)
     if e is None:
         e = _ENTRIES[fn] = _Entry(fn)
-    block = e.pack(*vals)
+    try:
+        block = e.pack(*vals)
+    except struct.error as err:
+        raise ValueError(f"dig_{fn}: a size or pitch is larger than the kernels take ({err})") from None
     tr = TRACE
     if tr is not None:
         kw = dict(zip(e.slot, vals))

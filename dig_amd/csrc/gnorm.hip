@@ -1161,7 +1161,8 @@ extern "C" int dig_gn_act_ws(int P, int C, int groups, int bwd, int vec, int dty
     const int esize = dtype == DIG_BF16 ? 2 : 4;
     if (vec && (bwd ? bwd_one_block(block_geo(P, C, groups, esize, g), P, g, esize) : fwd_one_block(block_geo(P, C, groups, esize, g), esize))) return bwd ? C * 2 : 0;
     const Geo q = geo_any(P, C, groups, vec != 0);
-    return (bwd ? q.S * C * 2 + groups * 2 : 0) + groups * q.nch * q.S * 2;
+    const long long n = (bwd ? 2ll * q.S * C + 2ll * groups : 0) + 2ll * groups * q.nch * q.S;
+    return n < (1ll << 31) ? (int)n : DIG_EINVAL;
 }
 
 extern "C" int dig_gn_act(const dig_gn_act_args* a, void* stream) {
@@ -1171,11 +1172,14 @@ extern "C" int dig_gn_act(const dig_gn_act_args* a, void* stream) {
     DIG_CHECK(a->dtype == DIG_BF16 || a->dtype == DIG_F32, DIG_EINVAL, "gn_act: dtype %d", a->dtype);
     DIG_CHECK(!a->ss || (a->ss_off >= 0 && a->ss_ld >= a->ss_off + 2 * a->C), DIG_EINVAL, "gn_act: scale/shift rows of %d values at %d do not hold 2 x %d", a->ss_ld,
               a->ss_off, a->C);
+    DIG_CHECK(a->x_bs >= 0 && a->x_ld >= 0 && (!a->res || (a->res_bs >= 0 && a->res_ld >= 0)), DIG_EINVAL, "gn_act: negative pitch");
     const bool vec = a->C % 8 == 0 && a->x_bs % 8 == 0 && a->x_ld % 8 == 0 && aligned16(a->x) && aligned16(a->out) &&
                      (!a->res || (a->res_bs % 8 == 0 && a->res_ld % 8 == 0 && aligned16(a->res)));
     FwdP p{a->x, a->gamma, a->beta, a->ss, a->res, a->out, a->mean_rstd, a->ws, a->x_bs, a->x_ld, a->res_bs, a->res_ld, a->ss_ld, a->ss_off, wide_params(a->gamma, a->beta, a->ss, a->ss_ld, a->ss_off, a->C), a->eps, geo_any(a->P, a->C, a->groups, vec)};
     DIG_CHECK((long long)a->B * p.q.nch * p.q.S < (1ll << 31) && (long long)a->B * a->groups < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
-    DIG_CHECK(a->ws || dig_gn_act_ws(a->P, a->C, a->groups, 0, vec, a->dtype) == 0, DIG_EINVAL, "gn_act: this shape needs a workspace");
+    const int need = dig_gn_act_ws(a->P, a->C, a->groups, 0, vec, a->dtype);
+    DIG_CHECK(need >= 0, DIG_EINVAL, "gn_act: %d groups of %d channels need too large a workspace", a->groups, a->C);
+    DIG_CHECK(need == 0 || (a->ws && aligned16(a->ws)), DIG_EINVAL, "gn_act: this shape needs a workspace, on 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     if (a->dtype == DIG_BF16) return vec ? fwd_act<bf16, 8>(p, a->B, a->act, st) : fwd_act<bf16, 1>(p, a->B, a->act, st);
     return vec ? fwd_act<float, 8>(p, a->B, a->act, st) : fwd_act<float, 1>(p, a->B, a->act, st);
@@ -1190,6 +1194,9 @@ extern "C" int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream) {
               a->ss_ld, a->ss_off, a->C);
     const bool vec = a->C % 8 == 0 && a->x_bs % 8 == 0 && a->x_ld % 8 == 0 && a->dy_bs % 8 == 0 && a->dy_ld % 8 == 0 && aligned16(a->x) && aligned16(a->dy) &&
                      aligned16(a->dx);
+    DIG_CHECK(a->x_bs >= 0 && a->x_ld >= 0 && a->dy_bs >= 0 && a->dy_ld >= 0, DIG_EINVAL, "gn_act_bwd: negative pitch");
+    DIG_CHECK(dig_gn_act_ws(a->P, a->C, a->groups, 1, vec, a->dtype) >= 0, DIG_EINVAL, "gn_act_bwd: %d groups of %d channels need too large a workspace", a->groups, a->C);
+    DIG_CHECK(aligned16(a->ws), DIG_EINVAL, "gn_act_bwd: ws has to lie on 16 bytes");
     const Geo q = geo_any(a->P, a->C, a->groups, vec);
     float* part = a->ws;
     float* gpart = part + (size_t)a->B * q.S * a->C * 2;

@@ -1065,7 +1065,8 @@ extern "C" int dig_linear_act(const dig_linear_act_args* a, void* stream) {
     DIG_CHECK(shape_ok(a->M, a->N, a->K), DIG_EINVAL, "linear_act: bad shape M=%d N=%d K=%d", a->M, a->N, a->K);
     DIG_CHECK(a->act >= 0 && a->act <= 3, DIG_EINVAL, "linear_act: act %d", a->act);
     DIG_CHECK(a->dtype == DIG_BF16 || a->dtype == DIG_F32, DIG_EINVAL, "linear_act: dtype %d", a->dtype);
-    DIG_CHECK(a->ws || dig_linear_act_ws(a->M, a->N, a->K, a->dtype) == 0, DIG_EINVAL, "linear_act: this shape needs a workspace");
+    DIG_CHECK(a->ldx >= 0 && a->ldw >= 0 && (!a->res || a->ldr >= 0), DIG_EINVAL, "linear_act: negative pitch");
+    DIG_CHECK((a->ws && al16(a->ws)) || dig_linear_act_ws(a->M, a->N, a->K, a->dtype) == 0, DIG_EINVAL, "linear_act: this shape needs a workspace, on 16 bytes");
     return a->dtype == DIG_BF16 ? fwd<bf16>(a, (hipStream_t)stream) : fwd<float>(a, (hipStream_t)stream);
 }
 
@@ -1075,5 +1076,7 @@ extern "C" int dig_linear_act_bwd(const dig_linear_act_bwd_args* a, void* stream
     DIG_CHECK(a->act >= 0 && a->act <= 3, DIG_EINVAL, "linear_act_bwd: act %d", a->act);
     DIG_CHECK(a->dtype == DIG_BF16 || a->dtype == DIG_F32, DIG_EINVAL, "linear_act_bwd: dtype %d", a->dtype);
     DIG_CHECK(a->act == ACT_NONE || (a->pre && a->dz), DIG_EINVAL, "linear_act_bwd: an activation needs pre and dz");
+    DIG_CHECK(a->ldx >= 0 && a->ldw >= 0 && a->ldy >= 0 && (a->act == ACT_NONE || a->ldpre >= 0), DIG_EINVAL, "linear_act_bwd: negative pitch");
+    DIG_CHECK(al16(a->ws) && al16(a->dz), DIG_EINVAL, "linear_act_bwd: ws and dz have to lie on 16 bytes");
     return a->dtype == DIG_BF16 ? bwd<bf16>(a, (hipStream_t)stream) : bwd<float>(a, (hipStream_t)stream);
 }

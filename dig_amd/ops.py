@@ -335,6 +335,12 @@ def _gn_check(who, x, gamma, beta, groups, ss, ss_off):
     return dev, B, C, P, dt
 
 
+def _ss_ld(ss):
+    if ss is None:
+        return 0
+    return ss.stride(0) if ss.shape[0] > 1 else ss.shape[1]
+
+
 @functools.lru_cache(maxsize=1024)
 def _gn_ws(P, C, groups, bwd, vec, dt):
     return _lib.lib().dig_gn_act_ws(P, C, groups, bwd, vec, dt)
@@ -366,9 +372,11 @@ def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off
     xp, op = x.data_ptr(), out.data_ptr()
     vec = not (C % 8 or (x_bs | x_ld | r_bs | r_ld) % 8 or (xp | op | rp) % 16)
     n = _gn_ws(P, C, groups, 0, vec, dt)
+    if n < 0:
+        raise ValueError(f"{who}: x {tuple(x.shape)} in {groups} groups is larger than the kernels take")
     ws = gamma.new_empty(B * n) if n else None
     _lib.launch("gn_act", dev, xp, gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, rp, op, mr.data_ptr(), ws.data_ptr() if n else 0,
-                x_bs, x_ld, r_bs, r_ld, B, P, C, groups, ss.stride(0) if ss is not None else 0, ss_off, code, dt, eps)
+                x_bs, x_ld, r_bs, r_ld, B, P, C, groups, _ss_ld(ss), ss_off, code, dt, eps)
     return (out, mr) if want_stats else out
 
 

@@ -120,10 +120,12 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     xp, dp, op = x.data_ptr(), dy.data_ptr(), dx.data_ptr()
     vec = not (C % 8 or (x_bs | x_ld | d_bs | d_ld) % 8 or (xp | dp | op) % 16)
     n = ops._gn_ws(P, C, groups, 1, vec, dt)
+    if n < 0:
+        raise ValueError(f"{who}: x {tuple(x.shape)} in {groups} groups is larger than the kernels take")
     ws = gamma.new_empty(B * n)
     launch("gn_act_bwd", dev, xp, dp, mean_rstd.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, op, dgamma.data_ptr(),
            dbeta.data_ptr(), dss.data_ptr() if ss is not None else 0, ws.data_ptr(), x_bs, x_ld, d_bs, d_ld, B, P, C, groups,
-           ss.stride(0) if ss is not None else 0, ss_off, code, dt)
+           ops._ss_ld(ss), ss_off, code, dt)
     return dx, dgamma, dbeta, dss
 
 

@@ -810,7 +810,7 @@ int dig_kd_bin_grad(const dig_kd_bin_grad_args* a, void* stream);
  * C % groups == 0, any alignment (16-byte aligned rows with C % 8 == 0 take 16-byte accesses).
  *   gamma, beta [C];  ss: per image row b * ss_ld + ss_off: scale [C] | shift [C], or NULL;  act: DIG_ACT_*
  *   mean_rstd [B][groups][2]: written, what the backward needs;  ws: B * dig_gn_act_ws(P, C, groups, 0, vec, dtype) floats, NULL
- *   when that is 0; vec: whether all rows are 16-byte aligned as above */
+ *   when that is 0; vec: whether all rows are 16-byte aligned as above.  Pitches are not negative; every workspace lies on 16 bytes */
 #define DIG_ACT_NONE 0
 #define DIG_ACT_RELU 1
 #define DIG_ACT_GELU 2 /* erf form */
@@ -858,7 +858,8 @@ int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream);
  * x [M][K] row pitch ldx, w [N][K] row pitch ldw, res [M][N] row pitch ldr (elements); bias [N] fp32 or NULL; out, pre [M][N]
  * contiguous (pre NULL: not kept); act: DIG_ACT_*.  Any M, N, K, pitch and alignment.  An operand whose rows do not lie on 16 bytes (its pointer, its
  * pitch, or K not a multiple of 8 - fp32: 4) or whose pitch reaches 2^31 / 256 bytes is copied to xpack [M][Kp] / wpack [N][Kp] first, Kp = K rounded
- * up to 16 bytes; otherwise xpack / wpack may be NULL.  ws: dig_linear_act_ws(...) floats (may be NULL when that is 0). */
+ * up to 16 bytes; otherwise xpack / wpack may be NULL.  ws: dig_linear_act_ws(...) floats (may be NULL when that is 0).  Pitches are
+ * not negative; every workspace lies on 16 bytes. */
 typedef struct {
     const void* x;
     const void* w;

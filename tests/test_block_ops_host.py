@@ -26,6 +26,9 @@ class _Fake(torch.Tensor):
         return 0
 
 
+LAUNCH = _lib.launch  # the tests below put a refusal in its place
+
+
 def F(*shape, dtype=torch.float32):
     return _Fake(torch.zeros(*shape, dtype=dtype))
 
@@ -165,3 +168,52 @@ def test_linear_act_c_entry_refuses():
             a.ldx = 17
             assert f(ctypes.byref(a), None) == -2 and b"need xpack" in L.dig_last_error()
     assert L.dig_linear_act_ws(0, 8, 8, 0) < 0 and L.dig_linear_act_bwd_ws(4, 0, 8, 0, 1) < 0
+
+
+def test_c_entries_refuse_pitches_and_workspaces():
+    """negative pitches, workspaces off 16 bytes, and sizes whose workspace does not fit 31 bits"""
+    L = _lib.lib()
+    for fn, shape, pitches, ws in (("gn_act", dict(B=2, P=1 << 20, C=16, groups=4, act=3), ("x_bs", "x_ld", "res_bs", "res_ld"), b"on 16 bytes"),
+                                   ("gn_act_bwd", dict(B=2, P=1 << 20, C=16, groups=4, act=3), ("x_bs", "x_ld", "dy_bs", "dy_ld"), b"on 16 bytes"),
+                                   ("linear_act", dict(M=16, N=64, K=8192), ("ldx", "ldw", "ldr"), b"on 16 bytes"),
+                                   ("linear_act_bwd", dict(M=16, N=64, K=64, act=1), ("ldx", "ldw", "ldy", "ldpre"), b"on 16 bytes")):
+        S = _lib.STRUCTS[f"dig_{fn}_args"]
+        f = getattr(L, f"dig_{fn}")
+        a = S()
+        for name, t in S._fields_:
+            if t is ctypes.c_void_p and name not in ("ss", "dss"):
+                setattr(a, name, 16)
+        for k, v in shape.items():
+            setattr(a, k, v)
+        for k in pitches:
+            setattr(a, k, -8)
+            assert f(ctypes.byref(a), None) == -1 and b"negative pitch" in L.dig_last_error(), (fn, k)
+            setattr(a, k, 64)
+        a.ws = 24
+        assert f(ctypes.byref(a), None) == -1 and ws in L.dig_last_error(), (fn, L.dig_last_error())
+    for bwd in (0, 1):
+        assert L.dig_gn_act_ws(1 << 20, 1 << 20, 1 << 20, bwd, 0, 1) < 0
+    S = _lib.STRUCTS["dig_gn_act_args"]
+    a = S()
+    for name, t in S._fields_:
+        if t is ctypes.c_void_p and name not in ("ss", "res"):
+            setattr(a, name, 16)
+    a.B, a.P, a.C, a.groups, a.dtype = 1, 1 << 20, 1 << 20, 1 << 20, 1
+    a.x_ld = 1 + (1 << 20)  # rows off 16 bytes
+    assert L.dig_gn_act(ctypes.byref(a), None) == -1 and b"too large a workspace" in L.dig_last_error()
+
+
+def test_sizes_beyond_31_bits_are_refused():
+    with pytest.raises(ValueError, match="larger than the kernels take"):
+        LAUNCH("gn_act", 0, *([0] * 8), *([0] * 4), 1, 1 << 32, *([0] * 6), 1e-5)
+
+
+def test_array_fields_do_not_run_into_the_next():
+    for fn in sorted(_lib.STRUCTS):
+        for name, t in _lib.STRUCTS[fn]._fields_:
+            n = getattr(t, "_length_", 0)
+            if n and fn.startswith("dig_") and fn.endswith("_args") and hasattr(_lib.lib(), fn[:-5]):
+                with pytest.raises(IndexError, match="holds"):
+                    _lib.call(fn[4:-5], **{name: [0] * (n + 1)})
+                return
+    pytest.skip("no argument block holds an array")
