@@ -450,7 +450,7 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> __global
 
 // ---- few outputs: a block takes 32 x 32 of them, its four waves every fourth K step.  The fragments come straight from memory (the operands are
 // small and shared through L2), all of a wave's loads for 4 steps in flight; the partial sums meet in LDS.  No k slices over blocks, so
-// one launch: 20x384x1536 fp32 takes ... ALIGNED as above; otherwise value by value.
+// one launch.  20x1536x384 with GELU and pre: 4.1 us in bf16, 6.9 in fp32.  ALIGNED: rows of whole 16 bytes; otherwise value by value.
 template <typename T, bool ALIGNED> __global__ __launch_bounds__(256) void linear_small_kernel(LinP p, int ctiles) {
     using F = typename Ops<T>::F;
     constexpr int E = 16 / (int)sizeof(T), KK = Ops<T>::KK, OS = 36;
@@ -755,28 +755,31 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> int fwd_
     return DIG_OK;
 }
 
-#ifndef FORCE_TILE
-#define FORCE_TILE -1
-#endif
 enum { TILE_SMALL = 0, TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4 };
 // Tile and k slices of the forward: the least estimated time.  A block of a tile costs fill + k tiles * step us while its CU holds as many
-// blocks as fit (slots in all); measured at 5864x384x81, 6912x384x1536 and 8192x4096x4096 in bf16 (64: 7.2 / 35 / 527 us, 128: 12.8 / 27 / 324, 192x128: 17 /
-// 24.5 / 311, 256: 23 / 29 / 245); fp32 steps are the matrix units' own time.  Few outputs take linear_small_kernel; few outputs of a long
-// sum are cut into k slices of 64 x 64 tiles, whose join costs a launch and the partial sums' bytes.
+// blocks as fit (slots in all).  Measured, GELU with pre kept, us (in brackets what is taken):
+//   M x N x K              64     128   192x128   256 |  fp32: 64   128   192x128   256
+//   1024 x 1024 x 1024   [7.8]   13.7    18.0    32.6 |     [25]    73       109    276
+//   4096 x 1024 x 1024    20.6  [17.8]   22.4    35.8 |     [80]    75       111    268
+//   6912 x 1536 x  384    34.6   26.4   [24.1]   27.5 |      97    112       [95]   121
+//   6912 x  384 x 1536   [20.6]  24.0    28.8    43.7 |     [86]   104       155    389
+//   6272 x 4096 x 1024     104    77      76     [74] |     465   [475]      518    545
+//   8192 x 4096 x 4096     406   254     261    [223] |
+// 256 x 256 is not built for fp32: it won nowhere.  Few outputs take linear_small_kernel (20x1536x384: 4.1 against 5.5; fp32 6.9 against 12.2); few
+// outputs of a long sum are cut into k slices of 64 x 64 tiles, whose join costs a launch and the partial sums' bytes (256x256x8192: 11.8 against 25.6 uncut).
 int fwd_plan(int M, int N, int K, int dtype, int& splits) {
     struct Cost {
         int br, bc, slots;
         double fill, step, step_f32;
     };
-    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 14.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 7.0}};
+    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 14.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 0.0}};
     const bool f32 = dtype != DIG_BF16;
     const int nk = up(K, f32 ? 32 : 64);
     splits = 1;
-    if (FORCE_TILE >= 0) return FORCE_TILE;
     const long long small = (long long)up(M, 32) * up(N, 32);
     double best = small <= 512 ? (3.0 + up(K, f32 ? 256 : 512) * (f32 ? 1.5 : 1.2)) * (small <= 256 ? 1.0 : 1.6) : 1e30;
     int tile = TILE_SMALL;
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < (f32 ? 3 : 4); i++) {
         const double tiles = (double)up(M, cost[i].br) * up(N, cost[i].bc), full = tiles / cost[i].slots;
         double rounds = full <= 1.0 ? 1.0 : full + 0.4;
         if (full > 1.0 && rounds > (double)(long long)full + 1.0) rounds = (double)(long long)full + 1.0;
@@ -869,7 +872,8 @@ template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     switch (tile) {
         case TILE_64: return fwd_launch<T, 64, 64, 2, 2, 4, 2>(p, st);
         case TILE_192: return fwd_launch<T, 192, 128, 2, 2, 2, 2>(p, st);
-        case TILE_256: return fwd_launch<T, 256, 256, 2, 4, 2, 2>(p, st);
+        case TILE_256:
+            if constexpr (sizeof(T) == 2) return fwd_launch<T, 256, 256, 2, 4, 2, 2>(p, st);
         default: return fwd_launch<T, 128, 128, 2, 2, 2, 2>(p, st);
     }
 }

@@ -130,6 +130,19 @@ def test_backward_shapes(M, N, K, dtype):
         check_bwd(x, w, dy, pre if i else None, act, has_bias=i != 1, dw_f32=i == 2, need_dx=i != 3 or M % 2 == 0)
 
 
+@pytest.mark.parametrize("M,N,K", [(13302, 777, 33), (12711, 776, 72), (12800, 777, 64), (10347, 1153, 387), (9953, 1160, 1032), (10240, 1280, 384)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows(M, N, K, dtype):
+    """enough outputs for the largest tiles, with partial tiles on every side"""
+    x, w, b = rnd(M, K, seed=M, dtype=dtype), rnd(N, K, seed=N, scale=K ** -0.5, dtype=dtype), rnd(N, seed=K)
+    r = rnd(M, N, seed=M + 1, dtype=dtype)
+    for act in ("none", "gelu"):
+        _, pre = check_fwd(x, w, b, act, r)
+    check_fwd(x, w, None, "relu", None, want_pre=False)
+    check_bwd(x, w, r, pre, "gelu")
+    check_bwd(x, w, r, None, "none", dw_f32=True)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_and_alignment(dtype):
     """channel slices of wider rows (aligned and not), a weight inside a larger one, broadcast rows"""
