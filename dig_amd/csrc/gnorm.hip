@@ -987,9 +987,29 @@ template <typename T, int ACT, int IPT, int NB> __global__ __launch_bounds__(NB)
         each_row2<2, T, 8>(x, xstep, dy, dstep, n, write);
     }
 }
-__global__ __launch_bounds__(NT) void gn_bwd_params_kernel(BwdP p) {
-    __shared__ double sm[NT / 64][8][2];
-    gn_bwd_params(p, blockIdx.x, sm);
+// dgamma, dbeta from the S1, S2 that the blocks above left per image: 16 channels by 16 shares of the images, all loads of a share in flight
+__global__ __launch_bounds__(256) void gn_bwd_params_kernel(BwdP p) {
+    __shared__ double sm[16][16][2];
+    const int cx = threadIdx.x & 15, y = threadIdx.x >> 4, C = p.q.C, c = blockIdx.x * 16 + cx;
+    double ga = 0.0, gb = 0.0;
+    if (c < C) {
+#pragma unroll 4
+        for (int b = y; b < p.B; b += 16) {
+            const f32x2 v = *reinterpret_cast<const f32x2*>(p.part + ((size_t)b * C + c) * 2);
+            const double sc = p.ss ? 1.0 + (double)p.ss[(size_t)b * p.ss_ld + p.ss_off + c] : 1.0;
+            gb += sc * (double)v[0];
+            ga += sc * (double)v[1];
+        }
+    }
+    sm[y][cx][0] = ga;
+    sm[y][cx][1] = gb;
+    __syncthreads();
+    if (y < 2 && c < C) {
+        double t = 0.0;
+#pragma unroll
+        for (int k = 0; k < 16; k++) t += sm[k][cx][y];
+        (y ? p.dbeta : p.dgamma)[c] = (float)t;
+    }
 }
 
 // ================================================== host ==================================================
@@ -1109,10 +1129,7 @@ template <typename T, int ACT> int bwd_launch_vec(BwdP p, hipStream_t st, bool& 
         hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 0, SLAB_BT>), grid, dim3(SLAB_BT), 0, st, p, g);
     }
     if (p.B > 1) {  // part is [B][C][2] here: the gradients of the parameters over the images
-        BwdP r = p;
-        r.q.S = 1;
-        r.dss = nullptr;  // written by the blocks
-        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)((p.q.C + 7) / 8)), dim3(NT), 0, st, r);
+        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)((p.q.C + 15) / 16)), dim3(256), 0, st, p);
     }
     DIG_LAUNCH_CHECK("gn_act_bwd");
     return DIG_OK;
