@@ -661,6 +661,7 @@ __device__ __forceinline__ void linear_db(const float* part, float* db, int chun
     const int cx = threadIdx.x & 15, y = threadIdx.x >> 4, c = blk * 16 + cx;
     double s = 0.0;
     if (c < N)
+#pragma unroll 8
         for (int k = y; k < chunks; k += 16) s += (double)part[(size_t)k * N + c];
     sm[y][cx] = s;
     __syncthreads();
