@@ -547,9 +547,9 @@ template <typename T> __device__ __forceinline__ void pack1(const T* src, T* dst
     }
     *reinterpret_cast<f32x4*>(dst) = f32x4{__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]), __builtin_bit_cast(float, w[2]), __builtin_bit_cast(float, w[3])};
 }
-template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackP p) {
+template <typename T> __device__ __forceinline__ void linear_pack(const PackP& p, int blk) {
     constexpr int E = 16 / (int)sizeof(T);
-    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    long long i = (long long)blk * 256 + threadIdx.x;
     int which = 0;
     if (i >= p.n[0]) {
         i -= p.n[0];
@@ -560,6 +560,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(
     const int k = (int)(i - r * p.per_row) * E;
     pack1<T>((const T*)p.src[which] + r * p.ld[which] + k, (T*)p.dst[which] + i * E, p.K - k);
 }
+template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackP p) { linear_pack<T>(p, blockIdx.x); }
 
 // splits > 1: the partial products of a row's 8 columns, added in order, and the epilogue
 template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear_join(const LinP& p, int blk) {
@@ -586,6 +587,7 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear
         load_bias<FULL>(p, c, bias);
         epi8<T, ACT, FULL>(p, v, r, c, rv, bias);
     } else {
+#pragma unroll 4
         for (int k = 0; k < p.splits; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++)
@@ -597,63 +599,87 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear
 }
 template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) { linear_join<T, ACT, true>(p, blockIdx.x); }
 
-// ---- dz = dy act'(z), and the column sums of the unrounded dz: a block takes 256 V columns by RPB rows
+// ---- dz = dy act'(z), and the column sums of the unrounded dz.  A block takes `rows` rows of LP V columns: LP lanes (2^lg) side by side, the
+// other 256 / LP threads share the rows, four of them in flight.  One block of rows: its sums are db.
 struct DzP {
     const void *dy, *pre;
     long long ldy, ldpre;
     void* dz;       // [M][ldz], columns N .. ldz - 1 zero; NULL: only the sums
-    float* part;    // [row blocks][N], or NULL
-    int M, N, ldz, rows;
+    float* part;    // [row blocks][N] (or db), or NULL
+    int M, N, ldz, rows, cols, lg;  // cols: blocks of columns
 };
-template <typename T, int V, int ACT> __device__ __forceinline__ void linear_dz(const DzP& p, int bx, int by, float* sm) {  // sm: 4 rows of 64 V + 1
-    const int c = (bx * 64 + (threadIdx.x & 63)) * V, ty = threadIdx.x >> 6;
-    const int row0 = by * p.rows, row1 = min(p.M, row0 + p.rows), width = p.dz ? p.ldz : p.N;
+template <typename T, int V, int ACT> __device__ __forceinline__ void linear_dz(const DzP& p, int blk, float* sm) {  // sm: 4 rows of 64 V
+    const int by = blk / p.cols, bx = blk - by * p.cols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lp = 1 << p.lg, cx = lane & (lp - 1);
+    const int c = (bx * lp + cx) * V, rt = 256 >> p.lg, width = p.dz ? p.ldz : p.N;
+    const long long row0 = (long long)by * p.rows, row1 = row0 + p.rows < p.M ? row0 + p.rows : p.M;
     float s[V];
 #pragma unroll
     for (int j = 0; j < V; j++) s[j] = 0.f;
     if (c < width) {
-        for (int r = row0 + ty; r < row1; r += 4) {
-            float d[V];
-            if constexpr (V == 8) {
-                Frag<T> f;
-                frag_load<T>(f, (const T*)p.dy + (size_t)r * p.ldy + c);
+        constexpr int U = 4;
+        for (long long r0 = row0 + (wave << (6 - p.lg)) + (lane >> p.lg); r0 < row1; r0 += U * rt) {
+            Frag<T> fd[V == 8 ? U : 1], fp[V == 8 && ACT != ACT_NONE ? U : 1];
+            float d[U], z[U];
 #pragma unroll
-                for (int j = 0; j < 8; j++) d[j] = frag_get<T>(f, j);
-                if constexpr (ACT != ACT_NONE) {
-                    frag_load<T>(f, (const T*)p.pre + (size_t)r * p.ldpre + c);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) d[j] *= act_slope<T, ACT>(frag_get<T>(f, j));
+            for (int u = 0; u < U; u++) {
+                const long long r = r0 + u * rt;
+                d[u] = 0.f;
+                if (r < row1) {
+                    if constexpr (V == 8) {
+                        frag_load<T>(fd[u], (const T*)p.dy + r * p.ldy + c);
+                        if constexpr (ACT != ACT_NONE) frag_load<T>(fp[u], (const T*)p.pre + r * p.ldpre + c);
+                    } else if (c < p.N) {
+                        d[u] = to_f32<T>(((const T*)p.dy)[r * p.ldy + c]);
+                        if constexpr (ACT != ACT_NONE) z[u] = to_f32<T>(((const T*)p.pre)[r * p.ldpre + c]);
+                    }
                 }
-                if (p.dz) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) frag_set<T>(f, j, d[j]);
-                    frag_store<T>(f, (T*)p.dz + (size_t)r * p.ldz + c);
-                }
-            } else {
-                d[0] = 0.f;
-                if (c < p.N) {
-                    d[0] = to_f32<T>(((const T*)p.dy)[(size_t)r * p.ldy + c]);
-                    if constexpr (ACT != ACT_NONE) d[0] *= act_slope<T, ACT>(to_f32<T>(((const T*)p.pre)[(size_t)r * p.ldpre + c]));
-                }
-                if (p.dz) ((T*)p.dz)[(size_t)r * p.ldz + c] = from_f32<T>(d[0]);
             }
 #pragma unroll
-            for (int j = 0; j < V; j++) s[j] += d[j];
+            for (int u = 0; u < U; u++) {
+                const long long r = r0 + u * rt;
+                if (r >= row1) continue;
+                if constexpr (V == 8) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        v[j] = frag_get<T>(fd[u], j);
+                        if constexpr (ACT != ACT_NONE) v[j] *= act_slope<T, ACT>(frag_get<T>(fp[u], j));
+                        s[j] += v[j];
+                    }
+                    if (p.dz) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) frag_set<T>(fd[u], j, v[j]);
+                        frag_store<T>(fd[u], (T*)p.dz + r * p.ldz + c);
+                    }
+                } else {
+                    if constexpr (ACT != ACT_NONE)
+                        if (c < p.N) d[u] *= act_slope<T, ACT>(z[u]);
+                    if (p.dz) ((T*)p.dz)[r * p.ldz + c] = from_f32<T>(d[u]);
+                    s[0] += d[u];
+                }
+            }
         }
     }
     if (!p.part) return;
 #pragma unroll
-    for (int j = 0; j < V; j++) sm[ty * (64 * V + 1) + (threadIdx.x & 63) * V + j] = s[j];
+    for (int j = 0; j < V; j++)
+        for (int o = lp; o < 64; o <<= 1) s[j] += __shfl_xor(s[j], o, 64);
+    const int W = lp * V;
+    if (lane < lp) {
+#pragma unroll
+        for (int j = 0; j < V; j++) sm[wave * W + cx * V + j] = s[j];
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * V; i += 256) {
-        const int col = bx * 64 * V + i;
-        constexpr int W = 64 * V + 1;
-        if (col < p.N) p.part[(size_t)by * p.N + col] = (sm[i] + sm[W + i]) + (sm[2 * W + i] + sm[3 * W + i]);
+    for (int i = threadIdx.x; i < W; i += 256) {
+        const int col = bx * W + i;
+        if (col < p.N) p.part[(size_t)by * p.N + col] = (float)(((double)sm[i] + (double)sm[W + i]) + ((double)sm[2 * W + i] + (double)sm[3 * W + i]));
     }
 }
-template <typename T, int V, int ACT> __global__ __launch_bounds__(256) void linear_dz_kernel(DzP p) {
-    __shared__ float sm[4 * (64 * V + 1)];
-    linear_dz<T, V, ACT>(p, blockIdx.x, blockIdx.y, sm);
+// what the products need first, in one launch: the first nd blocks write dz, the others pack x and w
+template <typename T, int V, int ACT> __global__ __launch_bounds__(256) void linear_dz_kernel(DzP p, PackP pp, int nd) {
+    __shared__ float sm[4 * 64 * V];
+    if ((int)blockIdx.x < nd) linear_dz<T, V, ACT>(p, blockIdx.x, sm);
+    else linear_pack<T>(pp, (int)blockIdx.x - nd);
 }
 __device__ __forceinline__ void linear_db(const float* part, float* db, int chunks, int N, int blk) {
     // 16 lanes x 16 columns: 16 strides of the chunks, joined in LDS in fp64
@@ -679,13 +705,12 @@ struct BwdP {
     int n0, n1;                   // blocks of the first and of the first two segments (multiples of 8, so that block index modulo 8 stays the XCD)
     int w_first;                  // the segment with the longer blocks comes first
     DzP s;
-    int sx;                       // column blocks of the sums
 };
 template <typename T, int TL, int SV> __global__ __launch_bounds__(256, 2) void linear_bwd_kernel(BwdP p) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int id = blockIdx.x;
     if (id >= p.n1) {
-        if constexpr (SV > 0) linear_dz<T, SV, ACT_NONE>(p.s, (id - p.n1) % p.sx, (id - p.n1) / p.sx, reinterpret_cast<float*>(smem));
+        linear_dz<T, SV, ACT_NONE>(p.s, id - p.n1, reinterpret_cast<float*>(smem));
         return;
     }
     const bool first = id < p.n0;
@@ -903,6 +928,24 @@ double makespan(double n1, double b1, double n2, double b2, double slots) {
     }
     return best < 1e30 ? best : t1 + (n2 / slots + 1.0) * b2;
 }
+// Rows of a block of linear_dz (a function of M and N alone: the workspace depends on it): about 1024 blocks in all, at least 4 rows and at most
+// 256 per thread, one block of rows where that makes at most 32 per thread (8 times as many where rows of 8 k values are misaligned).  4 rows in flight and narrow rows side by side in a wave:
+// 15722 x 64 in fp32 took 24.6 us with 64 lanes across the columns whatever N is and one row in flight.
+int lanes_log(int width, int V) {
+    int lg = 0;
+    while (lg < 6 && (V << lg) < width) lg++;
+    return lg;
+}
+int dz_rows(int M, int N) {
+    const int V = N % 8 == 0 ? 8 : 1, lg = lanes_log(N, V), rt = 256 >> lg;
+    if (M <= 32 * rt) return M;
+    const int cols = up(N, V << lg), want = cols < 1024 ? 1024 / cols : 1;
+    int rows = up(M, want);
+    if (rows < 4 * rt) rows = 4 * rt;
+    if (rows > 256 * rt) rows = 256 * rt;
+    return rows;
+}
+int dz_chunks(int M, int N) { return up(M, dz_rows(M, N)); }
 // The least estimated time of one launch of both products.  A block costs fill + its k tiles * step us (measured on dx of 6912x1536x384 and
 // 6272x1024x4096 in bf16: tile 64 28 / 119 us, tile 128 23 / 82 us; fp32 steps are the matrix units' own time); what is split is written and read again as fp32.
 BwdPlan bwd_search(int M, int N, int K, int dtype, bool dx) {
@@ -911,17 +954,20 @@ BwdPlan bwd_search(int M, int N, int K, int dtype, bool dx) {
     const int bk = f32 ? 32 : 64, nkx = up(N, bk), nkw = up(M, bk);
     BwdPlan plan{128, 1, 1};
     double best = 1e30;
+    const bool one_chunk = dz_chunks(M, N) == 1;
     for (int tile = 64; tile <= 128; tile += 64) {
         const double fill = tile == 64 ? 2.5 : f32 ? 6.0 : 11.0, step = tile == 64 ? (f32 ? 0.95 : 0.58) : (f32 ? 3.6 : 1.1);
         const double tx = dx ? (double)up(M, tile) * up(K, tile) : 0.0, tw = (double)up(N, tile) * up(K, tile);
-        for (int a = 1; a <= 4; a++) {
+        for (int a : cuts) {
             if (a > 1 && (!dx || nkx < 4 * a || tx * a > 2048)) break;
             for (int b : cuts) {
                 if (b > 1 && (nkw < 4 * b || tw * b > 2048)) break;
-                const double bx = fill + up(nkx, a) * step, bw = fill + up(nkw, b) * step;
+                const double st = tx * a + tw * b <= 256.0 ? 0.8 * step : step;  // a block alone on its CU
+                const double bx = fill + up(nkx, a) * st, bw = fill + up(nkw, b) * st;
                 double t = !dx || bw >= bx ? makespan(tw * b, bw, tx * a, bx, 512.0) : makespan(tx * a, bx, tw * b, bw, 512.0);
                 if (a > 1) t += 8.0 * a * M * K / 4.5e6;
                 if (b > 1) t += 8.0 * b * N * K / 4.5e6;
+                if ((a > 1 || b > 1) && one_chunk) t += 4.0;  // db needs no join: this one is a launch of its own
                 if (t < best - 1e-9) {
                     best = t;
                     plan = {tile, a, b};
@@ -946,27 +992,21 @@ BwdPlan bwd_plan(int M, int N, int K, int dtype, bool dx) {
     return e.plan;
 }
 
-// rows of a block of the dz kernel: 128 blocks of rows, each thread at most 256 fp32 additions deep until the grid's limit
-int dz_rows(int M) {
-    int rows = (M + 127) / 128;
-    if (rows < 32) rows = 32;
-    if (rows > 1024) rows = 1024;
-    if ((long long)rows * 65535 < M) rows = (int)(((long long)M + 65534) / 65535);
-    return rows;
-}
-int dz_chunks(int M) { return (M + dz_rows(M) - 1) / dz_rows(M); }
-
 bool shape_ok(int M, int N, int K) {
-    return M > 0 && N > 0 && K > 0 && N <= (1 << 20) && K <= (1 << 20) && (long long)((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE) < (1 << 22) &&
+    return M > 0 && N > 0 && K > 0 && M <= (1 << 30) && N <= (1 << 20) && K <= (1 << 20) && (long long)((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE) < (1 << 22) &&
            (long long)((M + TILE - 1) / TILE) * ((K + TILE - 1) / TILE) < (1 << 22);
 }
 
-template <typename T, int ACT> void dz_launch(const DzP& d, bool vec, dim3 grid, hipStream_t st) {
-    if (vec) hipLaunchKernelGGL((linear_dz_kernel<T, 8, ACT>), grid, dim3(256), 0, st, d);
-    else hipLaunchKernelGGL((linear_dz_kernel<T, 1, ACT>), grid, dim3(256), 0, st, d);
+template <typename T, int ACT> void dz_launch(const DzP& d, const PackP& pp, int nd, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)(nd + (int)((pp.n[0] + pp.n[1] + 255) / 256)));
+    if (vec) hipLaunchKernelGGL((linear_dz_kernel<T, 8, ACT>), grid, dim3(256), 0, st, d, pp, nd);
+    else hipLaunchKernelGGL((linear_dz_kernel<T, 1, ACT>), grid, dim3(256), 0, st, d, pp, nd);
 }
 
-long long sum_floats(int M, int N) { return up(dz_chunks(M) * N, 4) * 4ll; }
+long long sum_floats(int M, int N) {
+    const long long chunks = dz_chunks(M, N);
+    return chunks > 1 ? (chunks * N + 3) / 4 * 4 : 0;
+}
 long long part_floats(const BwdPlan& q, int M, int N, int K, bool dx, long long& dx_floats) {
     dx_floats = dx && q.sx > 1 ? ((long long)q.sx * M * K + 3) / 4 * 4 : 0;
     return dx_floats + (q.sw > 1 ? (long long)q.sw * N * K : 0);
@@ -974,7 +1014,7 @@ long long part_floats(const BwdPlan& q, int M, int N, int K, bool dx, long long&
 
 template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) {
     const int E = 16 / (int)sizeof(T), es = (int)sizeof(T), M = a->M, N = a->N, K = a->K, ldz = up(N, 8) * 8;
-    const int chunks = dz_chunks(M);
+    const int chunks = dz_chunks(M, N);
     float* sums = a->ws;  // column sums of row blocks, then the partial products of dx and dW
     float* part = a->ws + sum_floats(M, N);
     PackP pp{};
@@ -983,17 +1023,16 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
               "linear_act_bwd: rows that do not lie on 16 bytes need xpack / wpack");
     const Operand z = a->dz ? Operand{a->dz, ldz} : Operand{a->dy, a->ldy};
     DIG_CHECK(z.ld % E == 0 && al16(z.p) && (a->dz || N % E == 0) && offsets_ok(z.ld, true, es), DIG_EALIGN, "linear_act_bwd: rows of dy that do not lie on 16 bytes need dz");
-    pack_launch<T>(pp, st);
-    const DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, a->db ? sums : nullptr, M, N, ldz, dz_rows(M)};
     const bool dvec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre)));
-    const int width = a->dz ? ldz : N, dcols = dvec ? up(width, 512) : up(width, 64);
-    if (a->dz) {
-        const dim3 grid((unsigned)dcols, (unsigned)chunks);
-        switch (a->act) {
-            case ACT_RELU: dz_launch<T, ACT_RELU>(d, dvec, grid, st); break;
-            case ACT_GELU: dz_launch<T, ACT_GELU>(d, dvec, grid, st); break;
-            case ACT_SILU: dz_launch<T, ACT_SILU>(d, dvec, grid, st); break;
-            default: dz_launch<T, ACT_NONE>(d, dvec, grid, st); break;
+    const int width = a->dz ? ldz : N, lg = lanes_log(width, dvec ? 8 : 1), dcols = up(width, (dvec ? 8 : 1) << lg);
+    const DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, !a->db ? nullptr : chunks == 1 ? a->db : sums, M, N, ldz, dz_rows(M, N), dcols, lg};
+    if (a->dz || pp.n[0] + pp.n[1]) {
+        const int nd = a->dz ? dcols * chunks : 0;
+        switch (a->dz ? a->act : ACT_NONE) {
+            case ACT_RELU: dz_launch<T, ACT_RELU>(d, pp, nd, dvec, st); break;
+            case ACT_GELU: dz_launch<T, ACT_GELU>(d, pp, nd, dvec, st); break;
+            case ACT_SILU: dz_launch<T, ACT_SILU>(d, pp, nd, dvec, st); break;
+            default: dz_launch<T, ACT_NONE>(d, pp, nd, dvec, st); break;
         }
     }
     const BwdPlan plan = bwd_plan(M, N, K, a->dtype, a->dx != nullptr);
@@ -1032,7 +1071,6 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
     p.n1 = nw + nx;
     const bool sum_here = a->db && !a->dz;
     p.s = d;
-    p.sx = dcols;
     const dim3 grid((unsigned)(p.n1 + (sum_here ? dcols * chunks : 0)));
     constexpr size_t lds = lds_of<128, 128, 4, 2, 2>(), lds64 = lds_of<64, 64, 4, 2, 2>();
     static_assert(lds <= 64 * 1024, "no attribute needed");
@@ -1044,7 +1082,7 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
         else hipLaunchKernelGGL((linear_bwd_kernel<T, 64, 1>), grid, dim3(256), lds64, st, p);
     }
     auto join_blocks = [](const LinP& q) { return q.splits > 1 ? (int)(((long long)q.R * up(q.C, 8) + 255) / 256) : 0; };
-    const int jw = join_blocks(p.w), jx = a->dx ? join_blocks(p.x) : 0, jd = a->db ? up(N, 16) : 0;
+    const int jw = join_blocks(p.w), jx = a->dx ? join_blocks(p.x) : 0, jd = a->db && chunks > 1 ? up(N, 16) : 0;
     if (jw + jx + jd) hipLaunchKernelGGL((linear_bwd_join_kernel<T>), dim3((unsigned)(jw + jx + jd)), dim3(256), 0, st, p.w, p.x, jw, jx, sums, a->db, chunks, N);
     DIG_LAUNCH_CHECK("linear_act_bwd");
     return DIG_OK;
@@ -1076,12 +1114,14 @@ extern "C" int dig_linear_act(const dig_linear_act_args* a, void* stream) {
 }
 
 extern "C" int dig_linear_act_bwd(const dig_linear_act_bwd_args* a, void* stream) {
-    DIG_CHECK(a && a->x && a->w && a->dy && a->dw && a->ws, DIG_EINVAL, "linear_act_bwd: null pointer");
+    DIG_CHECK(a && a->x && a->w && a->dy && a->dw, DIG_EINVAL, "linear_act_bwd: null pointer");
     DIG_CHECK(shape_ok(a->M, a->N, a->K) && shape_ok(a->N, a->K, 1), DIG_EINVAL, "linear_act_bwd: bad shape M=%d N=%d K=%d", a->M, a->N, a->K);
     DIG_CHECK(a->act >= 0 && a->act <= 3, DIG_EINVAL, "linear_act_bwd: act %d", a->act);
     DIG_CHECK(a->dtype == DIG_BF16 || a->dtype == DIG_F32, DIG_EINVAL, "linear_act_bwd: dtype %d", a->dtype);
     DIG_CHECK(a->act == ACT_NONE || (a->pre && a->dz), DIG_EINVAL, "linear_act_bwd: an activation needs pre and dz");
     DIG_CHECK(a->ldx >= 0 && a->ldw >= 0 && a->ldy >= 0 && (a->act == ACT_NONE || a->ldpre >= 0), DIG_EINVAL, "linear_act_bwd: negative pitch");
+    const int need = dig_linear_act_bwd_ws(a->M, a->N, a->K, a->dtype, a->dx != nullptr);
+    DIG_CHECK(need >= 0 && (need == 0 || a->ws), DIG_EINVAL, "linear_act_bwd: this shape needs a workspace");
     DIG_CHECK(al16(a->ws) && al16(a->dz), DIG_EINVAL, "linear_act_bwd: ws and dz have to lie on 16 bytes");
     return a->dtype == DIG_BF16 ? bwd<bf16>(a, (hipStream_t)stream) : bwd<float>(a, (hipStream_t)stream);
 }

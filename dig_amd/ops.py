@@ -418,11 +418,11 @@ def _linear_ws(M, N, K, dt):
     return _lib.lib().dig_linear_act_ws(M, N, K, dt)
 
 
-def _packed(t, p, rows, K, ld, e):
-    """Workspace for the 16-byte aligned copy (e values per 16 bytes) of an operand [rows, K] that the kernels cannot read as it lies, or None."""
+def _packed(p, rows, K, ld, e):
+    """Bytes for the 16-byte aligned copy (e values per 16 bytes) of an operand [rows, K] that the kernels cannot read as it lies; 0: they can."""
     if not (K % e or ld % e or p % 16 or ld * 4096 >= e << 31):
-        return None
-    return t.new_empty((rows, (K + e - 1) // e * e))
+        return 0
+    return rows * ((K + e - 1) // e) * 16
 
 
 def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
@@ -440,10 +440,10 @@ def linear_act(x, w, bias=None, act="none", res=None, want_pre=False):
         n = _linear_ws(M, N, K, dt)
         if n < 0:
             raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
-        ws = torch.empty(n, dtype=_F32, device=x.device) if n else None
         xp, wp, ldw, e = x.data_ptr(), w.data_ptr(), w.stride(0), 8 if dt == 0 else 4
-        xk, wk = _packed(x, xp, M, K, ldx, e), _packed(w, wp, N, K, ldw, e)
+        xb, wb = _packed(xp, M, K, ldx, e), _packed(wp, N, K, ldw, e)
+        work = x.new_empty((xb + wb + 4 * n) * e // 16) if xb or wb or n else None  # xpack | wpack | ws
+        at = work.data_ptr() if work is not None else 0
         _lib.launch("linear_act", dev, xp, wp, bias.data_ptr() if bias is not None else 0, res.data_ptr() if res is not None else 0, y.data_ptr(),
-                    pre.data_ptr() if want_pre else 0, xk.data_ptr() if xk is not None else 0, wk.data_ptr() if wk is not None else 0, ws.data_ptr() if n else 0,
-                    ldx, ldw, ldr, M, N, K, code, dt)
+                    pre.data_ptr() if want_pre else 0, at if xb else 0, at + xb if wb else 0, at + xb + wb if n else 0, ldx, ldw, ldr, M, N, K, code, dt)
     return (y, pre) if want_pre else y

@@ -153,14 +153,14 @@ def linear_act_bwd(x, w, dy, pre=None, act="none", need_dx=True, has_bias=True, 
     n = _linear_bwd_ws(M, N, K, dt, need_dx)
     if n < 0:
         raise ValueError(f"{who}: [{M}, {K}] x [{N}, {K}] is larger than the kernels take")
-    ws = torch.empty(n, dtype=F32, device=x.device)
     xp, wp, dp, ldw, e = x.data_ptr(), w.data_ptr(), dy.data_ptr(), w.stride(0), 8 if dt == 0 else 4
     # dz of its own with an activation, and where the rows of dy do not lie on 16 bytes
-    dz = x.new_empty((M, (N + 7) // 8 * 8)) if code or N % e or ldy % e or dp % 16 or ldy * 4096 >= e << 31 else None
-    xk, wk = ops._packed(x, xp, M, K, ldx, e), ops._packed(w, wp, N, K, ldw, e) if need_dx else None
+    zb = M * ((N + 7) // 8) * 128 // e if code or N % e or ldy % e or dp % 16 or ldy * 4096 >= e << 31 else 0
+    xb, wb = ops._packed(xp, M, K, ldx, e), ops._packed(wp, N, K, ldw, e) if need_dx else 0
+    work = x.new_empty((zb + xb + wb + 4 * n) * e // 16) if zb or xb or wb or n else None  # dz | xpack | wpack | ws
+    at = work.data_ptr() if work is not None else 0
     launch("linear_act_bwd", dev, xp, wp, dp, pre.data_ptr() if code else 0, dx.data_ptr() if need_dx else 0, dw.data_ptr(), db.data_ptr() if has_bias else 0,
-           dz.data_ptr() if dz is not None else 0, xk.data_ptr() if xk is not None else 0, wk.data_ptr() if wk is not None else 0, ws.data_ptr(), ldx, ldw, ldy, ldpre,
-           M, N, K, code, dt, int(dw_f32))
+           at if zb else 0, at + zb if xb else 0, at + zb + xb if wb else 0, at + zb + xb + wb if n else 0, ldx, ldw, ldy, ldpre, M, N, K, code, dt, int(dw_f32))
     return dx, dw, db
 
 

@@ -878,7 +878,7 @@ int dig_linear_act_ws(int M, int N, int K, int dtype);
 
 /* adjoint: dz = dy * act'(pre),  dx = dz w (NULL: not wanted),  dw = dz^T x (dtype, or fp32 if dw_f32),  db = column sums of dz, fp32
  * (NULL: no bias); all outputs contiguous.  dz: [M][N rounded up to 8] of dtype, workspace; may be NULL when act is DIG_ACT_NONE and the rows of dy
- * lie on 16 bytes with N a multiple of 8 (fp32: 4) values (dy is then multiplied as it lies).  xpack, wpack as above.  ws: dig_linear_act_bwd_ws(...) floats.
+ * lie on 16 bytes with N a multiple of 8 (fp32: 4) values (dy is then multiplied as it lies).  xpack, wpack as above.  ws: dig_linear_act_bwd_ws(...) floats (may be NULL when that is 0).
  * The residual's gradient is dy itself. */
 typedef struct {
     const void* x;

@@ -191,6 +191,8 @@ def test_c_entries_refuse_pitches_and_workspaces():
             setattr(a, k, 64)
         a.ws = 24
         assert f(ctypes.byref(a), None) == -1 and ws in L.dig_last_error(), (fn, L.dig_last_error())
+    for M in (1 << 30) + 1, (1 << 31) - 1:
+        assert L.dig_linear_act_ws(M, 8, 8, 0) < 0 and L.dig_linear_act_bwd_ws(M, 8, 8, 0, 1) < 0
     for bwd in (0, 1):
         assert L.dig_gn_act_ws(1 << 20, 1 << 20, 1 << 20, bwd, 0, 1) < 0
     S = _lib.STRUCTS["dig_gn_act_args"]
