@@ -6,7 +6,8 @@
 //   dscale = gamma S2 + beta S1,  dshift = S1.
 // Everything between the loads and the stores is fp32, sums across threads fp64; the only rounding to bf16 is the stored result.
 // No atomics: partial sums lie in the workspace and are added in a fixed order, and how an image is split depends on its own
-// size only, so a result does not depend on the batch it is computed in.
+// size only, so a result does not depend on the batch it is computed in - but for the backward of larger images, many of
+// which go to one block each while few are split (bwd_one_block).
 #include "act.hpp"
 
 namespace {
@@ -180,34 +181,62 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
         }
     }
     __syncthreads();
-    // groups that meet this chunk, one wave each: weighted mean, then M2 about it
-    const int c1 = min(q.C, c0 + q.CH), g0 = c0 / q.cg, g1 = (c1 - 1) / q.cg, lane = tid & 63;
-    for (int g = g0 + (tid >> 6); g <= g1; g += NT / 64) {
+    // groups that meet this chunk: weighted mean, then M2 about it.  A wave takes one, or all four share it where there is only one;
+    // a row y of the block stands for `base` rows of the image, or one more.
+    __shared__ double sm_w[NT / 64][2];
+    const int c1 = min(q.C, c0 + q.CH), g0 = c0 / q.cg, g1 = (c1 - 1) / q.cg, lane = tid & 63, wave = tid >> 6;
+    const int base = q.P / cycle, extra = q.P - base * cycle - row0;
+    const bool shared = g0 == g1;
+    for (int g = g0 + (shared ? 0 : wave); g <= g1; g += NT / 64) {
         const int lo = max(c0, g * q.cg) - c0, hi = min(c1, (g + 1) * q.cg) - c0, w = hi - lo;
+        // lanes x channels x rows without a division in the loop: narrow groups put 64 / w rows side by side
+        const int side = w < 64 ? 64 / w : 1, y0 = w < 64 ? lane / w : 0, e0 = w < 64 ? lane - y0 * w : lane, per = shared ? NT / 64 : 1;
+        const int yfirst = y0 + (shared ? wave * side : 0), ystep = side * per;
+        const bool in = y0 < side;
         double sn = 0.0, sm = 0.0;
-        for (int e = lane; e < q.R * w; e += 64) {
-            const int y = e / w, n = rows_of(q.P, row0 + y, cycle);
-            if (n == 0) continue;
-            sm += (double)n * (double)sm_mean[y * q.CH + lo + e - y * w];
-            sn += (double)n;
-        }
+        if (in)
+            for (int y = yfirst; y < q.R; y += ystep) {
+                const double n = (double)(base + (y < extra ? 1 : 0));
+                for (int e = e0; e < w; e += 64) {
+                    sm += n > 0.0 ? n * (double)sm_mean[y * q.CH + lo + e] : 0.0;
+                    sn += n;
+                }
+            }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             sm += __shfl_xor(sm, o, 64);
             sn += __shfl_xor(sn, o, 64);
         }
+        if (shared) {  // the loop is left by all waves together
+            if (lane == 0) {
+                sm_w[wave][0] = sm;
+                sm_w[wave][1] = sn;
+            }
+            __syncthreads();
+            sm = (sm_w[0][0] + sm_w[1][0]) + (sm_w[2][0] + sm_w[3][0]);
+            sn = (sm_w[0][1] + sm_w[1][1]) + (sm_w[2][1] + sm_w[3][1]);
+            __syncthreads();
+        }
         const double mean = sm / sn;
         double m2 = 0.0;
-        for (int e = lane; e < q.R * w; e += 64) {
-            const int y = e / w, n = rows_of(q.P, row0 + y, cycle);
-            if (n == 0) continue;
-            const int i = y * q.CH + lo + e - y * w;
-            const double d = (double)sm_mean[i] - mean;
-            m2 += (double)sm_m2[i] + (double)n * d * d;
-        }
+        if (in)
+            for (int y = yfirst; y < q.R; y += ystep) {
+                const double n = (double)(base + (y < extra ? 1 : 0));
+                if (n > 0.0)
+                    for (int e = e0; e < w; e += 64) {
+                        const int i = y * q.CH + lo + e;
+                        const double d = (double)sm_mean[i] - mean;
+                        m2 += (double)sm_m2[i] + n * d * d;
+                    }
+            }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m2 += __shfl_xor(m2, o, 64);
-        if (lane == 0) {
+        if (shared) {
+            if (lane == 0) sm_w[wave][0] = m2;
+            __syncthreads();
+            m2 = (sm_w[0][0] + sm_w[1][0]) + (sm_w[2][0] + sm_w[3][0]);
+        }
+        if (lane == 0 && (!shared || wave == 0)) {
             float* d = p.part + (((size_t)b * q.G + g) * (q.nch * q.S) + ch * q.S + s) * 2;
             d[0] = (float)mean;
             d[1] = (float)m2;
@@ -1062,7 +1091,16 @@ constexpr int SLAB_MAX = 512 << 10;  // bytes of x that one block of the backwar
 
 // whether the one-block forms take a shape of n vectors per thread
 bool fwd_one_block(int n, int esize) { return n > 0 && n <= (esize == 2 ? 32 : 16); }
-bool bwd_one_block(int n, int P, const BGeo& g, int esize) { return n > 0 && (n <= (esize == 2 ? 16 : 8) || (long long)P * g.LP * 8 * esize <= SLAB_MAX); }
+// The backward's takes the time of one block, whose rows every thread walks through twice, the split passes a fixed part and then that of the
+// data: up to 8 vectors per thread the block is ahead for any batch.  Above, bf16: 8 x 2000x64 (16 blocks) 22.6 against 14.7 us, 8x1024x512 (64) 23.2
+// against 19.0, 16x1024x512 (128) 27.0 against 27.4; slabs read twice: 32x4096x64 (64) 44 against 27, fp32 (128) 43 against 35, 32x4096x256 (256) 78
+// against 86, 256x5215x16 (256) 41 against 64.
+constexpr int BWD_ALWAYS = 8;
+bool bwd_one_block(int n, int B, int P, const BGeo& g, int esize) {
+    if (n <= BWD_ALWAYS) return n > 0;
+    const long long blocks = (long long)B * g.nch;
+    return n <= (esize == 2 ? 16 : 8) ? blocks >= 128 : (long long)P * g.LP * 8 * esize <= SLAB_MAX && blocks >= 192;
+}
 
 template <typename T, int ACT> int fwd_launch_vec(const FwdP& p, int B, hipStream_t st, bool& done) {
     BGeo g;
@@ -1115,7 +1153,7 @@ template <typename T, int ACT> int bwd_launch_vec(BwdP p, hipStream_t st, bool& 
     BGeo g;
     const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
     const int most = sizeof(T) == 2 ? 16 : 8;
-    done = bwd_one_block(n, p.q.P, g, (int)sizeof(T));
+    done = bwd_one_block(n, p.B, p.q.P, g, (int)sizeof(T));
     if (!done) return DIG_OK;
     DIG_CHECK((long long)p.B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
     const dim3 grid((unsigned)(p.B * g.nch));
@@ -1176,7 +1214,8 @@ extern "C" int dig_gn_act_ws(int P, int C, int groups, int bwd, int vec, int dty
     if (!shape_ok(1, P, C, groups) || (vec && C % 8)) return DIG_EINVAL;
     BGeo g;
     const int esize = dtype == DIG_BF16 ? 2 : 4;
-    if (vec && (bwd ? bwd_one_block(block_geo(P, C, groups, esize, g), P, g, esize) : fwd_one_block(block_geo(P, C, groups, esize, g), esize))) return bwd ? C * 2 : 0;
+    const int per_thread = vec ? block_geo(P, C, groups, esize, g) : 0;
+    if (bwd ? per_thread > 0 && per_thread <= BWD_ALWAYS : fwd_one_block(per_thread, esize)) return bwd ? C * 2 : 0;
     const Geo q = geo_any(P, C, groups, vec != 0);
     const long long n = (bwd ? 2ll * q.S * C + 2ll * groups : 0) + 2ll * groups * q.nch * q.S;
     return n < (1ll << 31) ? (int)n : DIG_EINVAL;

@@ -165,6 +165,18 @@ def test_backward_shapes(B, P, C, G, dtype):
         check_bwd(x, mr, gamma, beta, rnd(B, P, C, seed=77 + i, dtype=dtype), act, ss=ss)
 
 
+@pytest.mark.parametrize("B,P,C,G", [(64, 1500, 64, 8), (100, 3000, 64, 8), (200, 2100, 24, 3), (130, 700, 48, 3), (7, 700, 48, 3), (260, 40, 8, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_images(B, P, C, G, dtype):
+    """batches whose backward gives a block a whole image, beside small ones of the same images"""
+    x, gamma, beta, ss = make(B, P, C, dtype, seed=B + P)
+    dy = rnd(B, P, C, seed=B, dtype=dtype)
+    for act in ("silu", "relu"):
+        _, mr = check_fwd(x, gamma, beta, G, act, ss=ss)
+        check_bwd(x, mr, gamma, beta, dy, act, ss=ss)
+    check_bwd(x[:3], mr[:3].contiguous(), gamma, beta, dy[:3], "gelu", ss=ss[:3])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_and_alignment(dtype):
     """channel slices of a wider tensor (aligned and not), every second image, a broadcast dy, ss rows inside a wider table"""
