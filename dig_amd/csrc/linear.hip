@@ -785,24 +785,29 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> int fwd_
     return DIG_OK;
 }
 
-enum { TILE_SMALL = 0, TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4 };
+enum { TILE_SMALL = 0, TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4, TILE_64_SHORT = 5 };
 // Tile and k slices of the forward: the least estimated time.  A block of a tile costs fill + k tiles * step us while its CU holds as many
-// blocks as fit (slots in all).  Measured, GELU with pre kept, us (in brackets what is taken):
-//   M x N x K              64     128   192x128   256 |  fp32: 64   128   192x128   256
+// blocks as fit (slots in all).  Measured, GELU with pre kept (last three: not kept), us, in brackets what is taken; "short" are 64 x 64 tiles with two
+// stages in LDS instead of four, four blocks per CU instead of two: ahead for many tiles of few k, behind (43 to 41 and 477 to 466) otherwise:
+//   M x N x K              64     128   192x128   256 |  fp32: 64   128   192x128   256  short
 //   1024 x 1024 x 1024   [7.8]   13.7    18.0    32.6 |     [25]    73       109    276
-//   4096 x 1024 x 1024    20.6  [17.8]   22.4    35.8 |     [80]    75       111    268
-//   6912 x 1536 x  384    34.6   26.4   [24.1]   27.5 |      97    112       [95]   121
+//   4096 x 1024 x 1024    20.6  [17.8]   22.4    35.8 |      80    [75]      111    268
+//   6912 x 1536 x  384    34.6   26.4   [24.1]   27.5 |      97    112        95    121   [90]
 //   6912 x  384 x 1536   [20.6]  24.0    28.8    43.7 |     [86]   104       155    389
 //   6272 x 4096 x 1024     104    77      76     [74] |     465   [475]      518    545
 //   8192 x 4096 x 4096     406   254     261    [223] |
+//   9409 x  408 x  168                                |      32     41        38          [27]
+//  30001 x   96 x   48                                |    16.9   18.9      25.3        [13.5]
+//  12288 x 1000 x  800                                |     184             [174]
 // 256 x 256 is not built for fp32: it won nowhere.  Few outputs take linear_small_kernel (20x1536x384: 4.1 against 5.5; fp32 6.9 against 12.2); few
 // outputs of a long sum are cut into k slices of 64 x 64 tiles, whose join costs a launch and the partial sums' bytes (256x256x8192: 11.8 against 25.6 uncut).
 int fwd_plan(int M, int N, int K, int dtype, int& splits) {
     struct Cost {
         int br, bc, slots;
-        double fill, step, step_f32;
+        double fill, step, alone;  // alone: a step where no CU holds two blocks
     };
-    static const Cost cost[] = {{64, 64, 512, 4.5, 0.445, 0.9}, {128, 128, 512, 7.4, 1.15, 3.5}, {192, 128, 512, 14.0, 1.5, 5.25}, {256, 256, 256, 19.2, 1.61, 0.0}};
+    static const Cost cost16[] = {{64, 64, 512, 4.5, 0.445, 0.445}, {128, 128, 512, 7.4, 1.15, 1.15}, {192, 128, 512, 14.0, 1.5, 1.5}, {256, 256, 256, 19.2, 1.61, 1.61}};
+    static const Cost cost32[] = {{64, 64, 512, 5.5, 1.0, 0.57}, {128, 128, 512, 16.0, 3.8, 1.83}, {192, 128, 512, 19.7, 6.2, 2.82}, {64, 64, 1024, 10.0, 1.57, 1.57}};
     const bool f32 = dtype != DIG_BF16;
     const int nk = up(K, f32 ? 32 : 64);
     splits = 1;
@@ -810,14 +815,16 @@ int fwd_plan(int M, int N, int K, int dtype, int& splits) {
     const bool odd = K % (f32 ? 4 : 8) != 0;  // read value by value by linear_small_kernel, packed for the others: 501x333x777 in bf16 24 against 14 us
     double best = small <= 512 ? (3.0 + (odd ? 0.026 * K : up(K, f32 ? 256 : 512) * (f32 ? 1.5 : 1.2))) * (small <= 256 ? 1.0 : 1.6) : 1e30;
     int tile = TILE_SMALL;
-    for (int i = 0; i < (f32 ? 3 : 4); i++) {
-        const double tiles = (double)up(M, cost[i].br) * up(N, cost[i].bc), full = tiles / cost[i].slots;
+    for (int i = 0; i < 4; i++) {
+        const Cost& c = f32 ? cost32[i] : cost16[i];
+        const double tiles = (double)up(M, c.br) * up(N, c.bc), full = tiles / c.slots;
+        if (f32 && i == 3 && (tiles <= 512.0 || nk > 12)) break;
         double rounds = full <= 1.0 ? 1.0 : full + 0.4;
         if (full > 1.0 && rounds > (double)(long long)full + 1.0) rounds = (double)(long long)full + 1.0;
-        const double t = rounds * (cost[i].fill + nk * (f32 ? cost[i].step_f32 : cost[i].step)) + (odd ? 4.0 : 0.0);
+        const double t = rounds * (c.fill + nk * (tiles <= 256.0 ? c.alone : c.step)) + (odd ? 4.0 : 0.0);
         if (t < best) {
             best = t;
-            tile = TILE_64 + i;
+            tile = f32 && i == 3 ? TILE_64_SHORT : TILE_64 + i;
         }
     }
     const long long t64 = (long long)up(M, 64) * up(N, 64);
@@ -902,6 +909,8 @@ template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     set_split(p, splits, KB / (int)sizeof(T));
     switch (tile) {
         case TILE_64: return fwd_launch<T, 64, 64, 2, 2, 4, 2>(p, st);
+        case TILE_64_SHORT:
+            if constexpr (sizeof(T) == 4) return fwd_launch<T, 64, 64, 2, 2, 2, 4>(p, st);
         case TILE_192: return fwd_launch<T, 192, 128, 2, 2, 2, 2>(p, st);
         case TILE_256:
             if constexpr (sizeof(T) == 2) return fwd_launch<T, 256, 256, 2, 4, 2, 2>(p, st);

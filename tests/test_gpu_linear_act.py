@@ -130,7 +130,7 @@ def test_backward_shapes(M, N, K, dtype):
         check_bwd(x, w, dy, pre if i else None, act, has_bias=i != 1, dw_f32=i == 2, need_dx=i != 3 or M % 2 == 0)
 
 
-@pytest.mark.parametrize("M,N,K", [(13302, 777, 33), (12711, 776, 72), (12800, 777, 64), (10347, 1153, 387), (9953, 1160, 1032), (10240, 1280, 384)])
+@pytest.mark.parametrize("M,N,K", [(13302, 777, 33), (12711, 776, 72), (12800, 777, 64), (10347, 1153, 387), (9953, 1160, 1032), (10240, 1280, 384), (9409, 408, 168), (30001, 97, 45)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_many_rows(M, N, K, dtype):
     """enough outputs for the largest tiles, with partial tiles on every side"""
