@@ -565,16 +565,17 @@ template <typename T> __device__ __forceinline__ void linear_pack(const PackP& p
 }
 template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackP p) { linear_pack<T>(p, blockIdx.x); }
 
-// splits > 1: the partial products of a row's 8 columns, added in order, and the epilogue
+// splits > 1: the partial products of a row's 8 columns (one column where rows are not stored as vectors: adjacent lanes on adjacent values),
+// added in order, and the epilogue.  8 columns per thread whatever the alignment: 5000x100x300 backward 29 us in bf16 and 42 in fp32, now 20 and 26.
 template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear_join(const LinP& p, int blk) {
-    const int cv = (p.C + 7) / 8;
     const long long i = (long long)blk * 256 + threadIdx.x;
-    if (i >= (long long)p.R * cv) return;
-    const int r = (int)(i / cv), c = (int)(i - (long long)r * cv) * 8, n = min(8, p.C - c);
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float* s = p.part + (size_t)r * p.C + c;
     const size_t step = (size_t)p.R * p.C;
-    if (p.vec) {  // n is 8
+    if (p.vec) {
+        const int cv = p.C / 8;
+        if (i >= (long long)p.R * cv) return;
+        const int r = (int)(i / cv), c = (int)(i - (long long)r * cv) * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const float* s = p.part + (size_t)r * p.C + c;
 #pragma unroll 4
         for (int k = 0; k < p.splits; k++) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(s + k * step), b = *reinterpret_cast<const f32x4*>(s + k * step + 4);
@@ -590,16 +591,16 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void linear
         load_bias<FULL>(p, c, bias);
         epi8<T, ACT, FULL>(p, v, r, c, rv, bias);
     } else {
-#pragma unroll 4
-        for (int k = 0; k < p.splits; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e < n) v[e] += s[k * step + e];
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < n) epi1<T, ACT, FULL>(p, v[e], r, c + e);
+        if (i >= (long long)step) return;
+        const int r = (int)(i / p.C), c = (int)(i - (long long)r * p.C);
+        float v = 0.f;
+        const float* s = p.part + i;
+#pragma unroll 8
+        for (int k = 0; k < p.splits; k++) v += s[k * step];
+        epi1<T, ACT, FULL>(p, v, r, c);
     }
 }
+inline long long join_blocks(const LinP& p) { return p.splits > 1 ? ((long long)p.R * (p.vec ? p.C / 8 : p.C) + 255) / 256 : 0; }
 template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) { linear_join<T, ACT, true>(p, blockIdx.x); }
 
 // ---- dz = dy act'(z), and the column sums of the unrounded dz.  A block takes `rows` rows of LP V columns: LP lanes (2^lg) side by side, the
@@ -773,7 +774,7 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> int fwd_
     const int rt = up(p.R, BR), ct = up(p.C, BC);
     hipLaunchKernelGGL(kern, dim3((unsigned)(rt * ct * p.splits)), dim3(WR * WC * 64), lds, st, p, rt, ct);
     if (p.splits > 1) {
-        const dim3 grid((unsigned)(((long long)p.R * up(p.C, 8) + 255) / 256));
+        const dim3 grid((unsigned)join_blocks(p));
         switch (p.act) {
             case ACT_RELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_RELU>), grid, dim3(256), 0, st, p); break;
             case ACT_GELU: hipLaunchKernelGGL((linear_join_kernel<T, ACT_GELU>), grid, dim3(256), 0, st, p); break;
@@ -1095,8 +1096,7 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
         if (sum_here && dvec) hipLaunchKernelGGL((linear_bwd_kernel<T, 64, 8>), grid, dim3(256), lds64, st, p);
         else hipLaunchKernelGGL((linear_bwd_kernel<T, 64, 1>), grid, dim3(256), lds64, st, p);
     }
-    auto join_blocks = [](const LinP& q) { return q.splits > 1 ? (int)(((long long)q.R * up(q.C, 8) + 255) / 256) : 0; };
-    const int jw = join_blocks(p.w), jx = a->dx ? join_blocks(p.x) : 0, jd = a->db && chunks > 1 ? up(N, 16) : 0;
+    const int jw = (int)join_blocks(p.w), jx = a->dx ? (int)join_blocks(p.x) : 0, jd = a->db && chunks > 1 ? up(N, 16) : 0;
     if (jw + jx + jd) hipLaunchKernelGGL((linear_bwd_join_kernel<T>), dim3((unsigned)(jw + jx + jd)), dim3(256), 0, st, p.w, p.x, jw, jx, sums, a->db, chunks, N);
     DIG_LAUNCH_CHECK("linear_act_bwd");
     return DIG_OK;
