@@ -363,21 +363,20 @@ template <int V> __device__ __forceinline__ void group_pairs(const float* pairs,
     }
 }
 
-// Factors of u = mul (x - mean) + add for the channels of a thread.  For bf16 tensors the mean is folded into add (one instruction less): that
-// costs U |mean| mul of absolute error in u (U = 2^-24), far below the step of x itself.  SiLU's factors are scaled by -log2 e (silu_pre).
+// Factors of u = mul (x - mean) + add for the channels of a thread.  The mean is taken off x first: folded into add (one instruction less) it would leave
+// U |mean| mul of absolute error (U = 2^-24), and mul goes up to 316 gamma' where a group is constant - xhat is 0 there and u has to be beta'.
+// SiLU's factors are scaled by -log2 e (silu_pre).
 template <typename T, int V, int ACT> struct Affine {
-    static constexpr bool FOLD = sizeof(T) == 2;
-    float mean[FOLD ? 1 : V], mul[V], add[V];
+    float mean[V], mul[V], add[V];
     __device__ __forceinline__ void set(int j, float m, float mu, float ad) {
-        if constexpr (FOLD) ad = fmaf(-m, mu, ad);
-        else mean[j] = m;
+        mean[j] = m;
         mul[j] = ACT == ACT_SILU ? mu * SILU_PRE : mu;
         add[j] = ACT == ACT_SILU ? ad * SILU_PRE : ad;
     }
     __device__ __forceinline__ float value(int j, float x) const {
-        if constexpr (!FOLD) x -= mean[j];
-        if constexpr (ACT == ACT_SILU) return silu_pre(mul[j], add[j], x);
-        else return act_val<T, ACT>(fmaf(x, mul[j], add[j]));
+        const float xc = x - mean[j];
+        if constexpr (ACT == ACT_SILU) return silu_pre(mul[j], add[j], xc);
+        else return act_val<T, ACT>(fmaf(xc, mul[j], add[j]));
     }
 };
 
