@@ -8,11 +8,17 @@
 // No atomics: partial sums lie in the workspace and are added in a fixed order, and how an image is split depends on its own
 // size only, so a result does not depend on the batch it is computed in - but for the backward of larger images, many of
 // which go to one block each while few are split (bwd_one_block).
+#include <type_traits>
+
 #include "act.hpp"
 
 namespace {
 
 constexpr int NT = 256;
+// Rows that a thread adds in fp32.  Where it has more than ROWS_MAX of them, it closes its sums every CHAIN rows and goes on in fp64 (LONG), in its own
+// place in LDS, so that the error does not grow with the image.  Not so below: the closing costs loads in flight (1x65536x512 bf16, 256 rows a thread: 55 us
+// unclosed, 69 closed, 55 over twice as many splits, see geo_of; 32x65536x64, 32 rows: 142 against 146).
+constexpr int ROWS_MAX = 64, CHAIN = 32;
 
 // V consecutive channels of one row as they lie in memory (V = 8: 16-byte aligned vectors; V = 1: any alignment)
 template <typename T, int V> struct Raw;
@@ -120,7 +126,8 @@ __host__ __device__ inline Geo geo_of(int P, int C, int G, int V, int rows_per_t
     q.CH = q.LP * V;
     q.nch = (C + q.CH - 1) / q.CH;
     int S = (P + q.R * rows_per_thread - 1) / (q.R * rows_per_thread);
-    if (S > 64) S = 64;
+    const int most = P > 64 * ROWS_MAX * q.R ? 128 : 64;
+    if (S > most) S = most;
     if (S < 1) S = 1;
     q.RS = (P + S - 1) / S;
     q.S = (P + q.RS - 1) / q.RS;
@@ -141,11 +148,14 @@ struct FwdP {
     Geo q;
 };
 
-// ---- pass 1: (mean, M2) of every (image, group, split): per-thread sums about the thread's own first sample.  A sum of n squares
-// about one of the samples is at most n + 1 times their M2, so the subtraction S2 - S1^2 / n loses at most about n ulps, whatever the mean.
+// ---- pass 1: (mean, M2) of every (image, group, split): per-thread sums about the thread's own first sample.  A sum of n squares about one of the
+// samples is at most n + 1 times their M2, so the subtraction S2 - S1^2 / n loses at most about n ulps, whatever the mean; n is at most ROWS_MAX.
+// LONG: runs of CHAIN rows, about the mean of the first 8 rows and later of all rows before the run.  With k rows behind the pivot, S2 of a run of n is at most
+// 1 + n / k (the first run) or 2 + n / k times the M2 of all these rows: 5 in the first run, 3 in the second, then less; runs are joined as (mean, M2) in fp64.
 // Bound by HBM: 32x65536x64 bf16 55 us = 4.9 TB/s.
-template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kernel(FwdP p) {
-    __shared__ float sm_mean[NT * V], sm_m2[NT * V];
+template <typename T, int V, bool LONG> __global__ __launch_bounds__(NT) void gn_stats_kernel(FwdP p) {
+    using Sum = std::conditional_t<LONG, double, float>;
+    __shared__ Sum sm_mean[NT * V], sm_m2[NT * V];
     const Geo q = p.q;
     int id = blockIdx.x;
     const int s = id % q.S;
@@ -158,27 +168,66 @@ template <typename T, int V> __global__ __launch_bounds__(NT) void gn_stats_kern
     if (on) {
         const int n = rows_of(q.P, row0 + ty, cycle);
         const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
+        const size_t step = (size_t)cycle * p.x_ld;
+        Sum *mean = sm_mean + ty * q.CH + tx * V, *m2 = sm_m2 + ty * q.CH + tx * V;
         float piv[V], s1[V], s2[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) piv[j] = s1[j] = s2[j] = 0.f;
-        each_row<8, T, V>(x, (size_t)cycle * p.x_ld, n, [&](const Raw<T, V>& v, int i) {
-            if (i == 0) {
+        for (int j = 0; j < V; j++) piv[j] = 0.f;
+        auto run = [&](int rows) {
 #pragma unroll
-                for (int j = 0; j < V; j++) piv[j] = v.get(j);
-            }
+            for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+            each_row<8, T, V>(x, step, rows, [&](const Raw<T, V>& v, int i) {
+                if (!LONG && i == 0) {
+#pragma unroll
+                    for (int j = 0; j < V; j++) piv[j] = v.get(j);
+                }
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float d = v.get(j) - piv[j];
+                    s1[j] += d;
+                    s2[j] = fmaf(d, d, s2[j]);
+                }
+            });
+            const float inv = rows > 0 ? 1.f / (float)rows : 0.f;
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float d = v.get(j) - piv[j];
-                s1[j] += d;
-                s2[j] = fmaf(d, d, s2[j]);
+                const float m = s1[j] * inv;
+                s2[j] -= s1[j] * m;
+                s1[j] = piv[j] + m;
             }
-        });
-        const float inv = n > 0 ? 1.f / (float)n : 0.f;
+        };
+        if constexpr (LONG) {  // n >= ROWS_MAX
+            Raw<T, V> v[8];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const float m = s1[j] * inv;
-            sm_mean[ty * q.CH + tx * V + j] = piv[j] + m;
-            sm_m2[ty * q.CH + tx * V + j] = s2[j] - s1[j] * m;
+            for (int u = 0; u < 8; u++) v[u].load(x + u * step);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                float t = 0.f;
+#pragma unroll
+                for (int u = 1; u < 8; u++) t += v[u].get(j) - v[0].get(j);
+                piv[j] = fmaf(t, 0.125f, v[0].get(j));
+            }
+            for (int done = 0; done < n;) {
+                const int rows = min(CHAIN, n - done);
+                run(rows);
+                x += rows * step;
+                const double w = (double)rows / (double)(done + rows), wd = w * (double)done;
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const double was = done ? mean[j] : 0.0, d = (double)s1[j] - was;
+                    mean[j] = was + d * w;
+                    m2[j] = (done ? m2[j] : 0.0) + (double)s2[j] + d * d * wd;
+                    piv[j] = (float)mean[j];
+                }
+                done += rows;
+            }
+        } else {
+            run(n);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                mean[j] = s1[j];
+                m2[j] = s2[j];
+            }
         }
     }
     __syncthreads();
@@ -1129,7 +1178,9 @@ template <typename T, int V, int ACT> int fwd_launch(const FwdP& p, int B, hipSt
     }
     const Geo& q = p.q;
     const int join = joins_in_block(q);
-    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)(B * q.nch * q.S)), dim3(NT), 0, st, p);
+    const dim3 cut((unsigned)(B * q.nch * q.S));
+    if ((q.P - 1) / (q.S * q.R) >= ROWS_MAX) hipLaunchKernelGGL((gn_stats_kernel<T, V, true>), cut, dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((gn_stats_kernel<T, V, false>), cut, dim3(NT), 0, st, p);
     if (!join) {
         const long long n = (long long)B * q.G;
         hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);

@@ -54,3 +54,42 @@ def test_constant_groups_far_from_zero(P, C, G, dtype):
             tol = tol + half(dtype) * (ref.abs() + tol)
         err = (y.double() - ref[:, None]).abs()
         assert float((err - tol[:, None]).max()) <= 0, (act, float(err.max()), float((err / tol[:, None]).max()))
+
+
+def stats64(x, G):
+    """mean and biased variance of [B, P, C] per image and group, a part of the pixels at a time"""
+    B, P, C = x.shape
+    parts = [x[:, i:i + 16384].double().reshape(B, -1, G, C // G) for i in range(0, P, 16384)] if x.numel() <= 1 << 27 else None
+    cut = lambda: parts if parts is not None else (x[:, i:i + 16384].double().reshape(B, -1, G, C // G) for i in range(0, P, 16384))  # noqa: E731
+    n = P * (C // G)
+    mean = sum(t.sum((1, 3)) for t in cut()) / n
+    return mean, sum((t - mean[:, None, :, None]).square().sum((1, 3)) for t in cut()) / n
+
+
+# rows that a thread adds: thousands (one row of 2048 channels at a time), hundreds, and of 30 channels that are no vectors
+@pytest.mark.parametrize("P,C,G,border", [(1 << 18, 2048, 8, 128), (65536, 1024, 8, 256), (1 << 17, 2048, 1, 300), (1 << 20, 30, 5, 4000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_statistics_of_many_rows(P, C, G, border, dtype):
+    """The first `border` rows, those that every thread begins with, lie 100 standard deviations off the rest.  A thread adds 32 fp32 values d = x - pivot
+    and their squares.  For a run of n values the sum of d is within n U sum |d| and that of d^2 within n U S2, so that M2 = S2 - S1^2 / n is within
+    n U S2 + 2 n U (sum |d|)^2 / n <= 3 n U S2.  A first run of 32 rows about the mean of its first 8 has S2 <= 5 M2: 480 U.  Those after it are about the mean of all k rows before,
+    so that S2 <= M2 + (1 + 32 / k) of what the run's mean adds to the variance, together at most 2 M2 of all rows: 192 U.  That is 672 U of the variance at most, half
+    of it for rstd (and 8 U for the rest: fp64 sums, their rounding, the stored value); the pivots' and the partial means' rounding (2 U of |x|) adds its square."""
+    x = rnd(1, 4096, C, seed=1, dtype=dtype).repeat(1, P // 4096, 1)
+    x += 100.0
+    x[:, :border] = 0.0
+    gamma, beta = rnd(C, seed=3, scale=0.3, shift=1.0), rnd(C, seed=4, scale=0.3)
+    y, mr = ops.group_norm_act(x, gamma, beta, groups=G, act="none", want_stats=True)
+    mean, var = stats64(x, G)
+    r = (var + 1e-5).rsqrt()
+    assert float(((mr[..., 0].double() - mean).abs() / mean.abs()).max()) <= 8 * U, "mean"
+    off = ((mr[..., 1].double() - r).abs() / r).max()
+    assert float(off) <= 344 * U + 4 * (100 * U * float(r.max())) ** 2, float(off) / U
+    for rows in (slice(0, 70), slice(P // 2 + 1, P // 2 + 40), slice(P - 70, P)):  # and what is made of them
+        rep = lambda t: t.repeat_interleave(C // G, 1)[:, None]  # noqa: E731
+        xh = (x[:, rows].double() - rep(mr[..., 0].double())) * rep(mr[..., 1].double())
+        ref = xh * gamma.double() + beta.double()
+        tol = 8 * U * ((xh * gamma).abs() + beta.abs())
+        if dtype != torch.float32:
+            tol = tol + half(dtype) * (ref.abs() + tol)
+        assert float(((y[:, rows].double() - ref).abs() - tol).max()) <= 0
