@@ -697,9 +697,10 @@ template <typename T, int ACT> __device__ __forceinline__ float du_of(const BwdP
     }
 }
 
-// ---- pass 1: per-channel sums of du and du xhat over the rows of a split
-template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(BwdP p) {
-    __shared__ float sm1[NT * V], sm2[NT * V];
+// ---- pass 1: per-channel sums of du and du xhat over the rows of a split.  LONG: a thread closes its sums every CHAIN rows.
+template <typename T, int V, int ACT, bool LONG> __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(BwdP p) {
+    using Sum = std::conditional_t<LONG, double, float>;
+    __shared__ Sum sm1[NT * V], sm2[NT * V];
     const Geo q = p.q;
     int id = blockIdx.x;
     const int s = id % q.S;
@@ -716,20 +717,30 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(NT) void gn_b
         for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
         const T* x = (const T*)p.x + (size_t)b * p.x_bs + (size_t)(row0 + ty) * p.x_ld + c;
         const T* dy = (const T*)p.dy + (size_t)b * p.d_bs + (size_t)(row0 + ty) * p.d_ld + c;
-        each_row2<4, T, V>(x, (size_t)q.R * p.x_ld, dy, (size_t)q.R * p.d_ld, rows_of(row1 - row0, ty, q.R), [&](const Raw<T, V>& vx, const Raw<T, V>& vd, int) {
+        const size_t xstep = (size_t)q.R * p.x_ld, dstep = (size_t)q.R * p.d_ld;
+        const int n = rows_of(row1 - row0, ty, q.R);
+        Sum *t1 = sm1 + ty * q.CH + tx * V, *t2 = sm2 + ty * q.CH + tx * V;
+        for (int done = 0;;) {
+            const int rows = LONG ? min(CHAIN, n - done) : n;
+            each_row2<4, T, V>(x, xstep, dy, dstep, rows, [&](const Raw<T, V>& vx, const Raw<T, V>& vd, int) {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
+                    s1[j] += du;
+                    s2[j] = fmaf(du, xc, s2[j]);
+                }
+            });
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float xv = vx.get(j), xc = xv - k[j].mean, du = du_of<T, ACT>(p, k[j], b, c + j, xv, xc, vd.get(j));
-                s1[j] += du;
-                s2[j] = fmaf(du, xc, s2[j]);
+                t1[j] = (LONG && done ? t1[j] : 0) + (Sum)s1[j];
+                t2[j] = (LONG && done ? t2[j] : 0) + (Sum)(s2[j] * k[j].rstd);
+                s1[j] = s2[j] = 0.f;
             }
-        });
-#pragma unroll
-        for (int j = 0; j < V; j++) s2[j] *= k[j].rstd;
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            sm1[ty * q.CH + tx * V + j] = s1[j];
-            sm2[ty * q.CH + tx * V + j] = s2[j];
+            if (!LONG) break;
+            done += rows;
+            if (done >= n) break;
+            x += rows * xstep;
+            dy += rows * dstep;
         }
     }
     __syncthreads();
@@ -1234,7 +1245,9 @@ template <typename T, int V, int ACT> int bwd_launch(const BwdP& p, hipStream_t 
         if (done) return rc;
     }
     const Geo& q = p.q;
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT>), dim3((unsigned)(p.B * q.nch * q.S)), dim3(NT), 0, st, p);
+    const dim3 cut((unsigned)(p.B * q.nch * q.S));
+    if ((q.RS - 1) / q.R >= ROWS_MAX) hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, true>), cut, dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, false>), cut, dim3(NT), 0, st, p);
     const int nparam = (q.C + 7) / 8;
     int S2, RS2;
     apply_split(q, p.B, S2, RS2);

@@ -93,3 +93,48 @@ def test_statistics_of_many_rows(P, C, G, border, dtype):
         if dtype != torch.float32:
             tol = tol + half(dtype) * (ref.abs() + tol)
         assert float(((y[:, rows].double() - ref).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("P,C,G", [(1 << 18, 2048, 8), (65536, 1024, 8), (1 << 20, 30, 5)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_sums_of_many_rows(P, C, G, act, dtype):
+    """Summands of one sign, so that no error cancels: a thread adds 32 of them in fp32 at a time, the rest is fp64 but for the stored sums of a split, S1, S2 and the gradients:
+    36 U of the sum of magnitudes, and 2 U more where (x - mean) rstd is a factor.  Slope of SiLU: |act''| <= 0.8, u good to 8 U of its terms, the functions
+    to (8 + 4 |u|) U of at most 1.13."""
+    x = rnd(1, 4096, C, seed=1, dtype=dtype).repeat(1, P // 4096, 1)
+    dy = rnd(1, 4096, C, seed=2, scale=0.05, shift=1.1, dtype=dtype).repeat(1, P // 4096, 1)
+    dy[:, :, ::3] = 1.1
+    gamma, beta = rnd(C, seed=3, scale=0.3, shift=1.0), rnd(C, seed=4, scale=0.3)
+    _, mr = ops.group_norm_act(x, gamma, beta, groups=G, act=act, want_stats=True)
+    dx, dgamma, dbeta, _ = train.group_norm_act_bwd(x, mr, gamma, beta, dy, act=act)
+    mean, r = (mr[0, :, k].double().repeat_interleave(C // G) for k in (0, 1))
+    a, b = gamma.double(), beta.double()
+
+    def terms(rows):
+        xh, d = (x[0, rows].double() - mean) * r, dy[0, rows].double()
+        if act == "none":
+            return xh, d, torch.zeros_like(d)
+        u = xh * a + b
+        sg = torch.sigmoid(u)
+        return xh, d * sg * (1 + u * (1 - sg)), d.abs() * U * (6.4 * ((xh * a).abs() + b.abs()) + 1.13 * (8 + 4 * u.abs()))
+
+    s1, s2, t1, t2 = (torch.zeros(C, dtype=torch.float64, device=DEV) for _ in range(4))
+    for xh, du, e in (terms(slice(i, i + 16384)) for i in range(0, P, 16384)):
+        s1 += du.sum(0)
+        s2 += (du * xh).sum(0)
+        t1 += (36 * U * du.abs() + e).sum(0)
+        t2 += ((38 * U * du.abs() + e) * xh.abs()).sum(0)
+    for name, got, ref, tol in (("dbeta", dbeta, s1, t1), ("dgamma", dgamma, s2, t2)):
+        err = (got.double() - ref).abs()
+        assert float((err - tol).max()) <= 0, (name, float((err / tol).max()))
+    group = lambda t: t.reshape(G, -1).sum(1).repeat_interleave(C // G) / (P * (C // G))  # noqa: E731
+    m1, m2, e1, e2 = group(s1 * a), group(s2 * a), group(t1 * a.abs()), group(t2 * a.abs())
+    for rows in (slice(0, 50), slice(P - 50, P)):
+        xh, du, e = terms(rows)
+        ref = r * (du * a - m1 - xh * m2)
+        tol = r * (e * a.abs() + 6 * U * ((du * a).abs() + m1.abs() + 2 * (xh * m2).abs()) + e1 + xh.abs() * e2) + 4 * U * ref.abs()
+        if dtype != torch.float32:
+            tol = tol + half(dtype) * (ref.abs() + tol)
+        err = (dx[0, rows].double() - ref).abs()
+        assert float((err - tol).max()) <= 0, ("dx", float((err / tol).max()))
