@@ -604,7 +604,8 @@ inline long long join_blocks(const LinP& p) { return p.splits > 1 ? ((long long)
 template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_join_kernel(LinP p) { linear_join<T, ACT, true>(p, blockIdx.x); }
 
 // ---- dz = dy act'(z), and the column sums of the unrounded dz.  A block takes `rows` rows of LP V columns: LP lanes (2^lg) side by side, the
-// other 256 / LP threads share the rows, four of them in flight.  One block of rows: its sums are db.  Bound by HBM: 6272x4096 bf16 with GELU 28 us =
+// other 256 / LP threads share the rows, four of them in flight.  A thread adds at most 256 values in fp32: dz_rows sees to that for vectors of 8 columns; value by
+// value (rows off 16 bytes) it has up to 8 times as many rows and goes on in fp64 after each 256.  One block of rows: its sums are db.  Bound by HBM: 6272x4096 bf16 with GELU 28 us =
 // 5.5 TB/s.
 struct DzP {
     const void *dy, *pre;
@@ -622,6 +623,8 @@ template <typename T, int V, int ACT> __device__ __forceinline__ void linear_dz(
     for (int j = 0; j < V; j++) s[j] = 0.f;
     if (c < width) {
         constexpr int U = 4;
+        double before = 0.0;
+        int added = 0;
         for (long long r0 = row0 + (wave << (6 - p.lg)) + (lane >> p.lg); r0 < row1; r0 += U * rt) {
             Frag<T> fd[V == 8 ? U : 1], fp[V == 8 && ACT != ACT_NONE ? U : 1];
             float d[U], z[U];
@@ -663,7 +666,14 @@ template <typename T, int V, int ACT> __device__ __forceinline__ void linear_dz(
                     s[0] += d[u];
                 }
             }
+            if constexpr (V == 1)
+                if ((added += U) == 256) {
+                    before += (double)s[0];
+                    s[0] = 0.f;
+                    added = 0;
+                }
         }
+        if constexpr (V == 1) s[0] = (float)(before + (double)s[0]);
     }
     if (!p.part) return;
 #pragma unroll
