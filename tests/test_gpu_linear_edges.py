@@ -37,3 +37,27 @@ def test_column_sums_of_rows_off_16_bytes(N):
     ref = ref * sg * (1 + z * (1 - sg))
     tol = 264 * U * ref.abs() + float(dy[0, 0]) * M * 1.13 * U * (8 + 4 * z.abs())
     assert float(((db.double() - ref).abs() - tol).max()) <= 0
+
+
+def test_every_row_counts_once():
+    """dw and db over 33 million rows of small whole numbers: every partial sum is below 2^24, so that the result is exact in any order"""
+    M, N, K = (1 << 25) + 128, 72, 72
+    bf = torch.bfloat16
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randint(-1, 2, (M, K), generator=g, device=DEV, dtype=torch.int8).to(bf)
+    wide = (torch.randint(0, 4, (M, N + 1), generator=g, device=DEV, dtype=torch.int8) == 3).to(bf)
+    w = rnd(N, K, seed=6, scale=0.1, dtype=bf)
+    for dy in (wide[:, :N].contiguous(), wide[:, 1:]):  # rows on 16 bytes and off them
+        dx, dw, db = train.linear_act_bwd(x, w, dy, dw_f32=True)
+        ref, cols = torch.zeros(N, K, dtype=torch.float64, device=DEV), torch.zeros(N, dtype=torch.float64, device=DEV)
+        for i in range(0, M, 1 << 22):
+            d, v = dy[i:i + (1 << 22)], x[i:i + (1 << 22)]
+            ref += d.double().t().contiguous() @ v.double()
+            cols += d.double().sum(0)
+        assert float(cols.max()) < 2 ** 24 and float(ref.abs().max()) < 2 ** 24
+        assert torch.equal(dw.double(), ref) and torch.equal(db.double(), cols)
+        for rows in (slice(0, 200), slice(M - 200, M)):
+            v, a = dy[rows].double() @ w.double(), dy[rows].double() @ w.double().abs()
+            tol = (N + 8) * U * a
+            assert float(((dx[rows].double() - v).abs() - tol - 2.0 ** -8 * (v.abs() + tol)).max()) <= 0
+        del dx, dw, db
