@@ -335,10 +335,15 @@ def _gn_check(who, x, gamma, beta, groups, ss, ss_off):
     return dev, B, C, P, dt
 
 
-def _ss_ld(ss):
+def _ss_rows(ss, ss_off, C):
+    """-> (ss, its row pitch, ss_off) as the kernels take them: rows that lie apart.  One row for all images (an expanded ss) is laid out first."""
     if ss is None:
-        return 0
-    return ss.stride(0) if ss.shape[0] > 1 else ss.shape[1]
+        return None, 0, 0
+    if ss.shape[0] == 1:
+        return ss, ss.shape[1], ss_off
+    if ss.stride(0) < ss_off + 2 * C:
+        ss, ss_off = ss[:, ss_off:ss_off + 2 * C].contiguous(), 0
+    return ss, ss.stride(0), ss_off
 
 
 @functools.lru_cache(maxsize=1024)
@@ -349,7 +354,7 @@ def _gn_ws(P, C, groups, bwd, vec, dt):
 def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off=0, res=None, eps=1e-5, want_stats=False):
     """act(GroupNorm(x) * (1 + scale) + shift) [+ res] of any channels-last tensor x [B, ..., C] (bf16 or fp32; rows of one pitch, e.g.
     a channel slice): Block.norm / scale-shift / act (ddp.py:158-166) where no conv3x3 left its statistics, any group count.
-    gamma, beta [C] fp32; ss [B, ld] fp32 rows holding (scale | shift) at ss_off; act: none | relu | gelu | silu; res like x.
+    gamma, beta [C] fp32; ss [B, ld] fp32 rows holding (scale | shift) at ss_off (one row may be expanded over the images); act: none | relu | gelu | silu; res like x.
     -> y contiguous, in x's type; with want_stats (y, mean_rstd [B, groups, 2] fp32), which train.group_norm_act_bwd takes."""
     who = "group_norm_act"
     dev, B, C, P, dt = _gn_check(who, x, gamma, beta, groups, ss, ss_off)
@@ -375,8 +380,9 @@ def group_norm_act(x, gamma, beta, groups=GN_GROUPS, act="silu", ss=None, ss_off
     if n < 0:
         raise ValueError(f"{who}: x {tuple(x.shape)} in {groups} groups is larger than the kernels take")
     ws = gamma.new_empty(B * n) if n else None
+    ss, ss_ld, ss_off = _ss_rows(ss, ss_off, C)
     _lib.launch("gn_act", dev, xp, gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, rp, op, mr.data_ptr(), ws.data_ptr() if n else 0,
-                x_bs, x_ld, r_bs, r_ld, B, P, C, groups, _ss_ld(ss), ss_off, code, dt, eps)
+                x_bs, x_ld, r_bs, r_ld, B, P, C, groups, ss_ld, ss_off, code, dt, eps)
     return (out, mr) if want_stats else out
 
 

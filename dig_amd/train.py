@@ -99,7 +99,7 @@ def layernorm_bwd(x, gamma, dy, add=None, eps=1e-6):
 
 def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_off=0):
     """Adjoint of ops.group_norm_act for x [B, ..., C] and the mean_rstd [B, groups, 2] it returned -> (dx like x, dgamma [C], dbeta [C],
-    dss [B, 2C] = (dscale | dshift) or None without ss), parameter gradients fp32.  The gradient of the residual is dy itself."""
+    dss [B, 2C] = (dscale | dshift) of each image, also where one row of ss is expanded over them, or None without ss), parameter gradients fp32.  The gradient of the residual is dy itself."""
     who = "group_norm_act_bwd"
     if mean_rstd.dim() != 3 or mean_rstd.shape[2] != 2 or mean_rstd.dtype != F32 or not mean_rstd.is_contiguous() or mean_rstd.shape[0] != x.shape[0]:
         raise ValueError(f"{who}: mean_rstd must be the contiguous float32 [B, groups, 2] of the forward, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
@@ -123,9 +123,10 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     if n < 0:
         raise ValueError(f"{who}: x {tuple(x.shape)} in {groups} groups is larger than the kernels take")
     ws = gamma.new_empty(B * n)
+    ss, ss_ld, ss_off = ops._ss_rows(ss, ss_off, C)
     launch("gn_act_bwd", dev, xp, dp, mean_rstd.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ss.data_ptr() if ss is not None else 0, op, dgamma.data_ptr(),
            dbeta.data_ptr(), dss.data_ptr() if ss is not None else 0, ws.data_ptr(), x_bs, x_ld, d_bs, d_ld, B, P, C, groups,
-           ops._ss_ld(ss), ss_off, code, dt)
+           ss_ld, ss_off, code, dt)
     return dx, dgamma, dbeta, dss
 
 

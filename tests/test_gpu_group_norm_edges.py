@@ -138,3 +138,27 @@ def test_gradient_sums_of_many_rows(P, C, G, act, dtype):
             tol = tol + half(dtype) * (ref.abs() + tol)
         err = (dx[0, rows].double() - ref).abs()
         assert float((err - tol).max()) <= 0, ("dx", float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_of_scale_and_shift_for_all_images(dtype):
+    """an expanded row (one time step for the whole batch) gives what its copies give, in a graph too; so do rows that overlap"""
+    B, P, C, G = 3, 50, 48, 6
+    x, dy, res = (rnd(B, P, C, seed=i, dtype=dtype) for i in (1, 2, 3))
+    gamma, beta, row = rnd(C, seed=4, shift=1.0), rnd(C, seed=5), rnd(1, 3 + 2 * C + 4, seed=6, scale=0.3)
+    for ss, off in ((row[:, :2 * C].expand(B, 2 * C), 0), (row.expand(B, -1), 3), (torch.as_strided(row, (B, 2 * C), (2, 1)), 0)):
+        def step(s, o):
+            y, mr = ops.group_norm_act(x, gamma, beta, groups=G, ss=s, ss_off=o, res=res, want_stats=True)
+            return (y, mr) + train.group_norm_act_bwd(x, mr, gamma, beta, dy, ss=s, ss_off=o)
+
+        got, want = step(ss, off), step(ss.contiguous(), off)
+        assert got[5].shape == (B, 2 * C) and all(torch.equal(p, q) for p, q in zip(got, want))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(ss, off)
+    for k in range(3):
+        row.copy_(rnd(*row.shape, seed=20 + k, scale=0.3))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs, step(ss.contiguous(), off))), k
