@@ -91,14 +91,14 @@ class _Entry:
     """dig_<fn> and how its argument block is packed: one struct.pack of all fields in order (the per-launch host cost is what bounds
     small batches: setting the fields of a ctypes structure one by one took longer than the rest of a call)."""
 
-    __slots__ = ("slot", "blank", "pack", "func", "sname")
+    __slots__ = ("slot", "blank", "pack", "func", "name", "sname")
 
     def __init__(self, fn):
         S = STRUCTS[_SNAME.get(fn, f"dig_{fn}_args")]
-        self.sname, self.slot, self.blank, fmt = S.__name__, {}, [], ""
+        self.name, self.sname, self.slot, self.blank, fmt = fn, S.__name__, {}, [], ""
         for name, t in S._fields_:
             n = getattr(t, "_length_", 0)
-            self.slot[name] = (len(self.blank), n)
+            self.slot[name] = (len(self.blank), n, t is ctypes.c_void_p)
             self.blank += [0] * (n or 1)
             fmt += _FMT[t._type_] * n if n else _FMT[t]
         packer = struct.Struct(fmt + "0q")  # native alignment, as the C compiler lays the fields out
@@ -107,6 +107,12 @@ class _Entry:
         self.pack = packer.pack
         self.func = lib()["dig_" + fn]  # a function object of its own: the block goes over as bytes
         self.func.argtypes, self.func.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+
+    def refuse(self, err):
+        """what struct.pack raised for a value that its field does not take, as the error of a call"""
+        if "required argument" in str(err):  # of another type than the field's
+            return TypeError(f"dig_{self.name}: a field of {self.sname} was given a value of the wrong type ({err})")
+        return ValueError(f"dig_{self.name}: a size or pitch is larger than the kernels take ({err})")
 
 
 _ENTRIES = {}
@@ -129,6 +135,10 @@ def call(fn, stream=None, **kw):
     vals = e.blank[:]
     slot = e.slot
     for k, v in kw.items():
+        at = slot.get(k)
+        if at is None:
+            raise TypeError(f"{e.sname} has no field {k!r}")
+        i, n, pointer = at
         if isinstance(v, torch.Tensor):
             if not v.is_cuda:
                 raise RuntimeError(f"dig_{fn}: argument {k!r} is a {v.device} tensor; the kernels take HIP-device pointers only "
@@ -138,19 +148,22 @@ def call(fn, stream=None, **kw):
                 dev = d
             elif d != dev:
                 raise RuntimeError(f"dig_{fn}: argument {k!r} lives on {d} but another argument on {dev}")
-            v = v.data_ptr()
-        at = slot.get(k)
-        if at is None:
-            raise TypeError(f"{e.sname} has no field {k!r}")
-        i, n = at
-        if n:
+            if not pointer:
+                raise TypeError(f"dig_{fn}: {k!r} is a number, not a tensor")
+            vals[i] = v.data_ptr()
+        elif n:
             v = tuple(v)
             if len(v) > n:
                 raise IndexError(f"dig_{fn}: {k!r} holds {n} values, got {len(v)}")
             vals[i:i + len(v)] = v
         elif v is not None:
             vals[i] = v
-    block = e.pack(*vals)
+        elif not pointer:
+            raise TypeError(f"dig_{fn}: {k!r} is a number, not None")
+    try:
+        block = e.pack(*vals)
+    except struct.error as err:
+        raise e.refuse(err) from None
     tr = TRACE
     if tr is not None:
         tr(fn, kw, 0)
@@ -177,7 +190,7 @@ def launch(fn, dev, *vals):
     try:
         block = e.pack(*vals)
     except struct.error as err:
-        raise ValueError(f"dig_{fn}: a size or pitch is larger than the kernels take ({err})") from None
+        raise e.refuse(err) from None
     tr = TRACE
     if tr is not None:
         kw = dict(zip(e.slot, vals))
