@@ -2,6 +2,9 @@
 #pragma once
 #include "common.hpp"
 
+// a launch holds fewer than 2^32 threads
+inline bool grid_fits(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
+
 enum { ACT_NONE = DIG_ACT_NONE, ACT_RELU = DIG_ACT_RELU, ACT_GELU = DIG_ACT_GELU, ACT_SILU = DIG_ACT_SILU };
 
 // Phi(u) of the standard normal and E = exp(-u^2 / 2): Phi(-a) = E erfcx(a / sqrt 2) / 2 with erfcx as a polynomial in t = 1 / (1 + 0.42 a / sqrt 2),

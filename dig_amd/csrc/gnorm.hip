@@ -1148,6 +1148,7 @@ bool joins_in_block(const Geo& q) {
     if (groups > q.G) groups = q.G;
     return groups <= JOIN_GROUPS && (long long)groups * q.nch * q.S <= JOIN_MAX;
 }
+long long join_blocks(long long pairs) { return (pairs + NT / 64 - 1) / (NT / 64); }
 bool read_once(long long bytes) { return bytes > (128ll << 20); }
 constexpr int SLAB_BT = 512;
 constexpr int SLAB_MAX = 512 << 10;  // bytes of x that one block of the backward reads twice
@@ -1170,7 +1171,7 @@ template <typename T, int ACT> int fwd_launch_vec(const FwdP& p, int B, hipStrea
     const int n = block_geo(p.q.P, p.q.C, p.q.G, (int)sizeof(T), g);
     done = fwd_one_block(n, (int)sizeof(T));
     if (!done) return DIG_OK;
-    DIG_CHECK((long long)B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act: too many blocks");
+    DIG_CHECK(grid_fits((long long)B * g.nch, BT), DIG_EINVAL, "gn_act: too many blocks");
     const dim3 grid((unsigned)(B * g.nch));
     if (n <= 2) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 2>), grid, dim3(BT), 0, st, p, g);
     else if (n <= 4) hipLaunchKernelGGL((gn_block_kernel<T, ACT, 4>), grid, dim3(BT), 0, st, p, g);
@@ -1189,12 +1190,13 @@ template <typename T, int V, int ACT> int fwd_launch(const FwdP& p, int B, hipSt
     }
     const Geo& q = p.q;
     const int join = joins_in_block(q);
+    DIG_CHECK(grid_fits((long long)B * q.nch * q.S, NT) && (join || grid_fits(join_blocks((long long)B * q.G), NT)), DIG_EINVAL, "gn_act: too many blocks");
     const dim3 cut((unsigned)(B * q.nch * q.S));
     if ((q.P - 1) / (q.S * q.R) >= ROWS_MAX) hipLaunchKernelGGL((gn_stats_kernel<T, V, true>), cut, dim3(NT), 0, st, p);
     else hipLaunchKernelGGL((gn_stats_kernel<T, V, false>), cut, dim3(NT), 0, st, p);
     if (!join) {
         const long long n = (long long)B * q.G;
-        hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);
+        hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)join_blocks(n)), dim3(NT), 0, st, p, n);
     }
     int S2, RS2;
     apply_split(q, B, S2, RS2);
@@ -1220,7 +1222,7 @@ template <typename T, int ACT> int bwd_launch_vec(BwdP p, hipStream_t st, bool& 
     const int most = sizeof(T) == 2 ? 16 : 8;
     done = bwd_one_block(n, p.B, p.q.P, g, (int)sizeof(T));
     if (!done) return DIG_OK;
-    DIG_CHECK((long long)p.B * g.nch < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
+    DIG_CHECK(grid_fits((long long)p.B * g.nch, BT), DIG_EINVAL, "gn_act_bwd: too many blocks");
     const dim3 grid((unsigned)(p.B * g.nch));
     if (n <= 2) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 2, BT>), grid, dim3(BT), 0, st, p, g);
     else if (n <= 4) hipLaunchKernelGGL((gn_bwd_block_kernel<T, ACT, 4, BT>), grid, dim3(BT), 0, st, p, g);
@@ -1245,18 +1247,16 @@ template <typename T, int V, int ACT> int bwd_launch(const BwdP& p, hipStream_t 
         if (done) return rc;
     }
     const Geo& q = p.q;
+    int S2, RS2;
+    apply_split(q, p.B, S2, RS2);
+    const int nparam = (q.C + 7) / 8, join = joins_in_block(q);
+    const long long pairs = (long long)p.B * q.G;
+    DIG_CHECK(grid_fits((long long)p.B * q.nch * q.S, NT) && grid_fits((long long)p.B * q.nch * S2 + nparam, NT) && (join || grid_fits(join_blocks(pairs), NT)), DIG_EINVAL,
+              "gn_act_bwd: too many blocks");
     const dim3 cut((unsigned)(p.B * q.nch * q.S));
     if ((q.RS - 1) / q.R >= ROWS_MAX) hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, true>), cut, dim3(NT), 0, st, p);
     else hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, false>), cut, dim3(NT), 0, st, p);
-    const int nparam = (q.C + 7) / 8;
-    int S2, RS2;
-    apply_split(q, p.B, S2, RS2);
-    const int join = joins_in_block(q);
-    if (!join) {
-        const long long n = (long long)p.B * q.G;
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)((n + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, st, p, n);
-    }
-    DIG_CHECK((long long)p.B * q.nch * S2 + nparam < (1ll << 31), DIG_EINVAL, "gn_act_bwd: too many blocks");
+    if (!join) hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)join_blocks(pairs)), dim3(NT), 0, st, p, pairs);
     const dim3 grid((unsigned)(p.B * q.nch * S2 + nparam));
     if (V == 8 && read_once(2ll * p.B * q.P * q.C * (long long)sizeof(T)))
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true>), grid, dim3(NT), 0, st, p, nparam, S2, RS2, join);

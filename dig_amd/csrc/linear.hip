@@ -874,10 +874,7 @@ template <typename T> bool operand(const void* src, long long ld, bool k_adjacen
     o = {pack, (long long)pp.per_row * E};
     return true;
 }
-template <typename T> void pack_launch(const PackP& pp, hipStream_t st) {
-    const long long n = pp.n[0] + pp.n[1];
-    if (n) hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, pp);
-}
+long long pack_blocks(const PackP& pp) { return (pp.n[0] + pp.n[1] + 255) / 256; }
 
 template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     const int E = 16 / (int)sizeof(T);
@@ -912,7 +909,8 @@ template <typename T> int fwd(const dig_linear_act_args* a, hipStream_t st) {
     Operand x, w;
     DIG_CHECK(operand<T>(a->x, a->ldx, true, a->M, a->K, a->xpack, pp, 0, x) && operand<T>(a->w, a->ldw, true, a->N, a->K, a->wpack, pp, 1, w), DIG_EALIGN,
               "linear_act: rows that do not lie on 16 bytes need xpack / wpack");
-    pack_launch<T>(pp, st);
+    DIG_CHECK(grid_fits(pack_blocks(pp), 256), DIG_EINVAL, "linear_act: too many blocks");
+    if (pack_blocks(pp)) hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)pack_blocks(pp)), dim3(256), 0, st, pp);
     p.p = x.p;
     p.q = w.p;
     p.ldp = x.ld;
@@ -1017,13 +1015,14 @@ BwdPlan bwd_plan(int M, int N, int K, int dtype, bool dx) {
     return e.plan;
 }
 
+// fewer than 2^22 tiles of 128 x 128: the grids of 64 x 64 tiles hold fewer than 2^32 threads, and block numbers fit an int
 bool shape_ok(int M, int N, int K) {
     return M > 0 && N > 0 && K > 0 && M <= (1 << 30) && N <= (1 << 20) && K <= (1 << 20) && (long long)((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE) < (1 << 22) &&
            (long long)((M + TILE - 1) / TILE) * ((K + TILE - 1) / TILE) < (1 << 22);
 }
 
 template <typename T, int ACT> void dz_launch(const DzP& d, const PackP& pp, int nd, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)(nd + (int)((pp.n[0] + pp.n[1] + 255) / 256)));
+    const dim3 grid((unsigned)(nd + pack_blocks(pp)));
     if (vec) hipLaunchKernelGGL((linear_dz_kernel<T, 8, ACT>), grid, dim3(256), 0, st, d, pp, nd);
     else hipLaunchKernelGGL((linear_dz_kernel<T, 1, ACT>), grid, dim3(256), 0, st, d, pp, nd);
 }
@@ -1051,15 +1050,6 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
     const bool dvec = N % 8 == 0 && a->ldy % 8 == 0 && al16(a->dy) && (a->act == ACT_NONE || (a->ldpre % 8 == 0 && al16(a->pre)));
     const int width = a->dz ? ldz : N, lg = lanes_log(width, dvec ? 8 : 1), dcols = up(width, (dvec ? 8 : 1) << lg);
     const DzP d{a->dy, a->pre, a->ldy, a->ldpre, a->dz, !a->db ? nullptr : chunks == 1 ? a->db : sums, M, N, ldz, dz_rows(M, N), dcols, lg};
-    if (a->dz || pp.n[0] + pp.n[1]) {
-        const int nd = a->dz ? dcols * chunks : 0;
-        switch (a->dz ? a->act : ACT_NONE) {
-            case ACT_RELU: dz_launch<T, ACT_RELU>(d, pp, nd, dvec, st); break;
-            case ACT_GELU: dz_launch<T, ACT_GELU>(d, pp, nd, dvec, st); break;
-            case ACT_SILU: dz_launch<T, ACT_SILU>(d, pp, nd, dvec, st); break;
-            default: dz_launch<T, ACT_NONE>(d, pp, nd, dvec, st); break;
-        }
-    }
     const BwdPlan plan = bwd_plan(M, N, K, a->dtype, a->dx != nullptr);
     long long xf;
     (void)part_floats(plan, M, N, K, a->dx != nullptr, xf);
@@ -1097,6 +1087,16 @@ template <typename T> int bwd(const dig_linear_act_bwd_args* a, hipStream_t st) 
     const bool sum_here = a->db && !a->dz;
     p.s = d;
     const dim3 grid((unsigned)(p.n1 + (sum_here ? dcols * chunks : 0)));
+    const int nd = a->dz ? dcols * chunks : 0;
+    DIG_CHECK(grid_fits(nd + pack_blocks(pp), 256) && grid_fits(grid.x, 256), DIG_EINVAL, "linear_act_bwd: too many blocks");
+    if (nd + pack_blocks(pp)) {
+        switch (a->dz ? a->act : ACT_NONE) {
+            case ACT_RELU: dz_launch<T, ACT_RELU>(d, pp, nd, dvec, st); break;
+            case ACT_GELU: dz_launch<T, ACT_GELU>(d, pp, nd, dvec, st); break;
+            case ACT_SILU: dz_launch<T, ACT_SILU>(d, pp, nd, dvec, st); break;
+            default: dz_launch<T, ACT_NONE>(d, pp, nd, dvec, st); break;
+        }
+    }
     constexpr size_t lds = lds_of<128, 128, 4, 2, 2>(), lds64 = lds_of<64, 64, 4, 2, 2>();
     static_assert(lds <= 64 * 1024, "no attribute needed");
     if (plan.tile == 128) {
