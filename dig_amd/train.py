@@ -101,7 +101,7 @@ def group_norm_act_bwd(x, mean_rstd, gamma, beta, dy, act="silu", ss=None, ss_of
     """Adjoint of ops.group_norm_act for x [B, ..., C] and the mean_rstd [B, groups, 2] it returned -> (dx like x, dgamma [C], dbeta [C],
     dss [B, 2C] = (dscale | dshift) of each image, also where one row of ss is expanded over them, or None without ss), parameter gradients fp32.  The gradient of the residual is dy itself."""
     who = "group_norm_act_bwd"
-    if mean_rstd.dim() != 3 or mean_rstd.shape[2] != 2 or mean_rstd.dtype != F32 or not mean_rstd.is_contiguous() or mean_rstd.shape[0] != x.shape[0]:
+    if mean_rstd.dim() != 3 or mean_rstd.shape[2] != 2 or mean_rstd.dtype != F32 or not mean_rstd.is_contiguous() or mean_rstd.shape[:1] != x.shape[:1]:
         raise ValueError(f"{who}: mean_rstd must be the contiguous float32 [B, groups, 2] of the forward, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
     groups = mean_rstd.shape[1]
     dev, B, C, P, dt = ops._gn_check(who, x, gamma, beta, groups, ss, ss_off)
