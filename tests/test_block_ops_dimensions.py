@@ -10,7 +10,7 @@ def test_no_dimensions():
         def get_device(self):
             return 0
 
-    f = lambda *shape: torch.zeros(*shape).as_subclass(OnDevice)  # noqa: E731
+    f = lambda *shape: torch.zeros(shape).as_subclass(OnDevice)  # noqa: E731
     with pytest.raises(ValueError, match="must be \\[B"):
         ops.group_norm_act(f(), f(16), f(16), groups=4)
     with pytest.raises(ValueError, match="mean_rstd must be"):
