@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from dig_amd import ops, train
+from dig_amd import _lib, ops, train
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -162,3 +162,42 @@ def test_one_row_of_scale_and_shift_for_all_images(dtype):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outs, step(ss.contiguous(), off))), k
+
+
+# 128 splits of an image, joined by the blocks that use them (8 groups) or by a launch of their own (32); vectors and single channels
+@pytest.mark.parametrize("P,C,G", [(20000, 512, 8), (40001, 256, 32), (50003, 30, 5), (70001, 24, 24)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_splits(P, C, G, dtype):
+    """buffers of the documented sizes and nothing behind them; the same image alone and in a batch; mean, rstd and the parameters' gradients in 64 bits (tolerances as above)"""
+    B, L, dt, vec = 2, _lib.lib(), 0 if dtype == torch.bfloat16 else 1, int(C % 8 == 0)
+    x, dy, gamma, beta = rnd(B, P, C, seed=1, shift=0.5, dtype=dtype), rnd(B, P, C, seed=2, dtype=dtype), rnd(C, seed=3, scale=0.3, shift=1.0), rnd(C, seed=4, scale=0.3)
+    y, mr = ops.group_norm_act(x, gamma, beta, groups=G, act="silu", want_stats=True)
+    grads = train.group_norm_act_bwd(x, mr, gamma, beta, dy, act="none")
+    y1, mr1 = ops.group_norm_act(x[1:], gamma, beta, groups=G, act="silu", want_stats=True)
+    assert torch.equal(y1, y[1:]) and torch.equal(mr1, mr[1:])
+    assert torch.equal(train.group_norm_act_bwd(x[1:], mr1, gamma, beta, dy[1:], act="none")[0], grads[0][1:])
+    mean, var = stats64(x, G)
+    r = (var + 1e-5).rsqrt()
+    assert float((mr[..., 0].double() - mean).abs().max()) <= 8 * U * float(x.double().abs().max())
+    assert float(((mr[..., 1].double() - r).abs() / r).max()) <= 344 * U
+    rep = lambda t: t.double().repeat_interleave(C // G, 1)[:, None]  # noqa: E731
+    xh = (x.double() - rep(mr[..., 0])) * rep(mr[..., 1])
+    d = dy.double()
+    for got, t, n in ((grads[1], d * xh, 38), (grads[2], d, 36)):
+        assert float(((got.double() - t.sum((0, 1))).abs() - n * U * t.abs().sum((0, 1))).max()) <= 0
+    guard = 16384
+
+    def buf(n, t=torch.float32):
+        b = torch.full((n + guard,), 7.0, dtype=t, device=DEV)
+        b[:n] = float("nan")
+        return b
+
+    at = dict(x=x, gamma=gamma, beta=beta, x_bs=P * C, x_ld=C, B=B, P=P, C=C, groups=G, dtype=dt)
+    out, m2, w1, w2 = buf(B * P * C, dtype), buf(2 * B * G), buf(B * L.dig_gn_act_ws(P, C, G, 0, vec, dt)), buf(B * L.dig_gn_act_ws(P, C, G, 1, vec, dt))
+    _lib.call("gn_act", out=out, mean_rstd=m2, ws=w1, act=3, eps=1e-5, **at)
+    dx, dg, db = buf(B * P * C, dtype), buf(C), buf(C)
+    _lib.call("gn_act_bwd", dy=dy, mean_rstd=mr, dx=dx, dgamma=dg, dbeta=db, ws=w2, dy_bs=P * C, dy_ld=C, act=0, **at)
+    torch.cuda.synchronize()
+    for b, want in ((out, y), (m2, mr), (dx, grads[0]), (dg, grads[1]), (db, grads[2]), (w1, None), (w2, None)):
+        assert bool((b[-guard:] == 7.0).all())
+        assert want is None or torch.equal(b[:-guard], want.reshape(-1))
