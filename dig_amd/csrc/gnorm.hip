@@ -4,7 +4,8 @@
 //   du = dy act'(u),  S1[b,c] = sum_p du,  S2[b,c] = sum_p du xhat,  m1 / m2 = group means of gamma' du / gamma' du xhat,
 //   dx = rstd (gamma' du - m1 - xhat m2),  dgamma = sum_b (1 + scale) S2,  dbeta = sum_b (1 + scale) S1,
 //   dscale = gamma S2 + beta S1,  dshift = S1.
-// Everything between the loads and the stores is fp32, sums across threads fp64; the only rounding to bf16 is the stored result.
+// Everything between the loads and the stores is fp32, sums across threads fp64, and a thread's own sums where they are long (LONG); a block's or a split's
+// sums are stored in fp32.  The only rounding to bf16 is the stored result.
 // No atomics: partial sums lie in the workspace and are added in a fixed order, and how an image is split depends on its own
 // size only, so a result does not depend on the batch it is computed in - but for the backward of larger images, many of
 // which go to one block each while few are split (bwd_one_block).
@@ -497,7 +498,7 @@ template <typename T, int V, int ACT, bool ONCE> __global__ __launch_bounds__(NT
 
 // ---- one launch: a block owns an image's groups g0 .. g0 + gpc - 1 and keeps all of their pixels in registers (IPT vectors of 8
 // channels per thread): x is read once, no partial sums, no second launch.  Per thread sums about its first row, as above, joined across the block.
-// 32x1024x512 bf16 20 us = 3.4 TB/s, the reading and the writing half one after the other (every block of the launch is resident); 1x16x128 5 us, latency.
+// 32x1024x512 bf16 20.4 us = 3.3 TB/s, the reading and the writing half one after the other (every block of the launch is resident); 1x16x128 5 us, latency.
 // Consecutive blocks go to the 8 XCDs in turn; the blocks of one image share 128-byte lines where a group's rows are shorter than that, so
 // each XCD (and its L2) gets a contiguous run of them.  Backward 32x4096x256, 64-byte rows: 104 us in plain order, 84 so.
 __device__ __forceinline__ int xcd_run(int id, int n) {
@@ -873,8 +874,8 @@ __device__ __forceinline__ float dx_of(float ga, float du, float rstd, float xc,
     return rstd * ((g - m1) - xc * rm2);
 }
 
-// ---- pass 2: the first nparam blocks finish the parameters' gradients, the others write dx; every block joins its groups itself
-// (order and ONCE as in gn_apply_kernel)
+// ---- pass 2: the first nparam blocks finish the parameters' gradients, the others write dx; as in the forward every block joins its groups itself where they
+// are few (join), otherwise gn_bwd_join_kernel has (order and ONCE as in gn_apply_kernel)
 template <typename T, int V, int ACT, bool ONCE> __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(BwdP p, int nparam, int S2, int RS2, int join) {
     __shared__ double sm_p[NT / 64][8][2];
     __shared__ float sm_m[2 * JOIN_GROUPS];

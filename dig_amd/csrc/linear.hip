@@ -167,9 +167,10 @@ template <typename T, bool TR, int X> __device__ __forceinline__ typename Ops<T>
 
 template <int N> __device__ __forceinline__ void dma_wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// Bound by the matrix units where k is long: 8192x4096x4096 bf16 with SiLU and residual 223 us = 1.23 PFLOP/s (a library product of that size alone takes
-// 203 us here); fp32 113 to 128 TFLOP/s of the 154 that one reaches, with the matrix units 81 % busy.  With few k tiles the first tile's latency and the
-// epilogue's stores are most of it: 6912x1536x384 with GELU and pre 24 us, of which the bytes are 10.
+// Bound by the matrix units where k is long: 8192x4096x4096 bf16 with SiLU and residual 239 us = 1.15 PFLOP/s, 223 on inputs that stay in the caches (a library
+// product of that size alone takes 203 us); fp32 127 TFLOP/s at 2048x2048x2048, 113 at 6272x4096x1024 and 95 at 6912x384x1536, of the 154 that a large library
+// product reaches.  The fp32 backward of 5864x1536x384 makes 100 TFLOP/s, its matrix units busy in 80 % of the CUs' busy cycles.  With few k tiles the first
+// tile's latency and the epilogue's stores are most of it: 6912x1536x384 with GELU and pre 22 us (24 traced), of which the bytes are 10.
 // Tile BR x BC, WR x WC waves.  Both operands have 16-byte aligned rows whose k (or own index) count fills them (the host packs others first).
 // FULL: the forward's epilogue.
 //
@@ -177,8 +178,8 @@ template <int N> __device__ __forceinline__ void dma_wait_barrier() { asm volati
 // pinned with sched_barrier: left alone, hipcc sinks the reads to their first use).  One barrier per tile of 128 bytes of k, before its
 // last K step: by then the wave holds the rest of the tile in registers, and the next tile is in LDS.
 // Both operands k-adjacent: NS tiles in LDS, filled by LDS-DMA; the place of a tile is filled again during its last K step.
-// Otherwise (TQ): two tiles in LDS, filled through registers, which fetch a tile ahead - hipcc waits for every DMA in flight before a transposing
-// read, so the two do not go together.
+// Otherwise (TQ): two tiles in LDS, filled through registers, which fetch a tile ahead: with the builtin for LDS-DMA hipcc waits for every DMA in flight
+// before a transposing read (a DMA issued from inline asm, which it does not track, has not been tried here).
 template <typename T, bool TP, bool TQ, int BR, int BC, int WR, int WC, int NS, bool FULL>
 __device__ __forceinline__ void linear_tile(const LinP& p, int rtiles, int ctiles, int id, unsigned char* smem) {
     using SP = Side<T, TP, BR>;
@@ -453,7 +454,7 @@ template <typename T, int BR, int BC, int WR, int WC, int NS, int MINW> __global
 
 // ---- few outputs: a block takes 32 x 32 of them, its four waves every fourth K step.  The fragments come straight from memory (the operands are
 // small and shared through L2), all of a wave's loads for 4 steps in flight; the partial sums meet in LDS.  No k slices over blocks, so
-// one launch.  20x1536x384 with GELU and pre: 4.1 us in bf16, 6.9 in fp32.  ALIGNED: rows of whole 16 bytes; otherwise value by value.
+// one launch.  20x1536x384 with GELU and pre: 4.7 us in bf16, 7.6 in fp32 (traced).  ALIGNED: rows of whole 16 bytes; otherwise value by value.
 template <typename T, bool ALIGNED> __global__ __launch_bounds__(256) void linear_small_kernel(LinP p, int ctiles) {
     using F = typename Ops<T>::F;
     constexpr int E = 16 / (int)sizeof(T), KK = Ops<T>::KK, OS = 36;
@@ -605,8 +606,8 @@ template <typename T, int ACT> __global__ __launch_bounds__(256) void linear_joi
 
 // ---- dz = dy act'(z), and the column sums of the unrounded dz.  A block takes `rows` rows of LP V columns: LP lanes (2^lg) side by side, the
 // other 256 / LP threads share the rows, four of them in flight.  A thread adds at most 256 values in fp32: dz_rows sees to that for vectors of 8 columns; value by
-// value (rows off 16 bytes) it has up to 8 times as many rows and goes on in fp64 after each 256.  One block of rows: its sums are db.  Bound by HBM: 6272x4096 bf16 with GELU 28 us =
-// 5.5 TB/s.
+// value (rows off 16 bytes) it has up to 8 times as many rows and goes on in fp64 after each 256.  One block of rows: its sums are db.  Bound by HBM:
+// 6272x4096 bf16 with GELU 29 us = 5.3 TB/s.
 struct DzP {
     const void *dy, *pre;
     long long ldy, ldpre;
@@ -810,7 +811,7 @@ enum { TILE_SMALL = 0, TILE_64 = 1, TILE_128 = 2, TILE_192 = 3, TILE_256 = 4, TI
 //   9409 x  408 x  168                                |      32     41        38          [27]
 //  30001 x   96 x   48                                |    16.9   18.9      25.3        [13.5]
 //  12288 x 1000 x  800                                |     184             [174]
-// 256 x 256 is not built for fp32: it won nowhere.  Few outputs take linear_small_kernel (20x1536x384: 4.1 against 5.5; fp32 6.9 against 12.2); few
+// 256 x 256 is not built for fp32: it won nowhere.  Few outputs take linear_small_kernel (20x1536x384, traced: 4.7 against 6.4; fp32 7.6 against 13.4); few
 // outputs of a long sum are cut into k slices of 64 x 64 tiles, whose join costs a launch and the partial sums' bytes (256x256x8192: 11.8 against 25.6 uncut).
 int fwd_plan(int M, int N, int K, int dtype, int& splits) {
     struct Cost {

@@ -810,7 +810,8 @@ int dig_kd_bin_grad(const dig_kd_bin_grad_args* a, void* stream);
  * C % groups == 0, any alignment (16-byte aligned rows with C % 8 == 0 take 16-byte accesses).
  *   gamma, beta [C];  ss: per image row b * ss_ld + ss_off: scale [C] | shift [C], or NULL;  act: DIG_ACT_*
  *   mean_rstd [B][groups][2]: written, what the backward needs;  ws: B * dig_gn_act_ws(P, C, groups, 0, vec, dtype) floats, NULL
- *   when that is 0; vec: whether all rows are 16-byte aligned as above.  Pitches are not negative; every workspace lies on 16 bytes */
+ *   when that is 0; vec: whether all rows are 16-byte aligned as above.  Pitches are not negative; every workspace lies on 16 bytes.
+ *   P <= 2^30, C <= 2^20, and fewer than 2^32 threads a launch: fewer than 2^23 images of one block each, of larger ones fewer yet */
 #define DIG_ACT_NONE 0
 #define DIG_ACT_RELU 1
 #define DIG_ACT_GELU 2 /* erf form */
@@ -856,7 +857,8 @@ int dig_gn_act_bwd(const dig_gn_act_bwd_args* a, void* stream);
  * mctformer.py:89-93,163-164; ddp.py:180,194), in a form that can be trained:
  *   pre = x w^T + bias,  out = act(pre) [+ res]
  * x [M][K] row pitch ldx, w [N][K] row pitch ldw, res [M][N] row pitch ldr (elements); bias [N] fp32 or NULL; out, pre [M][N]
- * contiguous (pre NULL: not kept); act: DIG_ACT_*.  Any M, N, K, pitch and alignment.  An operand whose rows do not lie on 16 bytes (its pointer, its
+ * contiguous (pre NULL: not kept); act: DIG_ACT_*.  Any pitch and alignment; N, K <= 2^20, M <= 2^30, and fewer than 2^22 tiles of 128 x 128 in
+ * [M][N], in [M][K] and (backward) in [N][K]: M < 2^29 where N and K are at most 128.  An operand whose rows do not lie on 16 bytes (its pointer, its
  * pitch, or K not a multiple of 8 - fp32: 4) or whose pitch reaches 2^31 / 256 bytes is copied to xpack [M][Kp] / wpack [N][Kp] first, Kp = K rounded
  * up to 16 bytes; otherwise xpack / wpack may be NULL.  ws: dig_linear_act_ws(...) floats (may be NULL when that is 0).  Pitches are
  * not negative; every workspace lies on 16 bytes. */
