@@ -18,7 +18,7 @@ namespace {
 constexpr int NT = 256;
 // Rows that a thread adds in fp32.  Where it has more than ROWS_MAX of them, it closes its sums every CHAIN rows and goes on in fp64 (LONG), in its own
 // place in LDS, so that the error does not grow with the image.  Not so below: the closing costs loads in flight (1x65536x512 bf16, 256 rows a thread: 55 us
-// unclosed, 69 closed, 55 over twice as many splits, see geo_of; 32x65536x64, 32 rows: 142 against 146).
+// unclosed, 69 closed, 50 closed over twice as many splits, see geo_of; 32x65536x64, 32 rows: 142 against 146).
 constexpr int ROWS_MAX = 64, CHAIN = 32;
 
 // V consecutive channels of one row as they lie in memory (V = 8: 16-byte aligned vectors; V = 1: any alignment)
@@ -110,7 +110,9 @@ __device__ __forceinline__ void each_row2(const T* p, size_t pstep, const T* d, 
     }
 }
 
-// How an image is cut: chunks of channels (LP lanes x V channels), R rows at a time in a block, S splits of RS rows.
+// How an image is cut: chunks of channels (LP lanes x V channels), R rows at a time in a block, S splits of RS rows: as many as leave a thread 8 rows, at
+// most 64, or 128 of images where a thread would have more than ROWS_MAX rows.  More splits cost their joins: 128 for 32x65536x64 bf16, 32 rows a thread in
+// 64, 156 us against 146; for 1x65536x512, 256 rows, they are ahead, 50 against 69 forward and 79 against 163 backward.
 struct Geo {
     int P, C, G, cg, LP, R, CH, nch, S, RS;
 };
